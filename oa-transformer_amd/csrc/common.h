@@ -112,16 +112,17 @@ OAT_DEV void gelu_both(float x, float& gl, float& dg) {
   dg = __builtin_fmaf(x * 0.3989422804f, e, cdf);
 }
 
-// ---- GELU of the bf16 GEMM epilogues (round 6): gelu(x) and gelu'(x) - 1/2 for TWO elements on packed fp32 math.
+// ---- GELU of the bf16 GEMM epilogues (round 6): gelu(x) and gelu'(x) - 1/2 for TWO elements side by side.
 // The fc1 epilogue is VALU-bound (the matrix pipe idles while a tile is finished: 12.5 of a K = 768 tile's 31 us), so what
 // counts is issue slots per element.  gelu_both above costs 20.75 (ISA count: two quarter-rate transcendentals = 8, the
-// A-S polynomial in t = 1 / (1 + p |x|), sign handling, 8-bit pack); this form costs 16:
+// A-S polynomial in t = 1 / (1 + p |x|), sign handling, 8-bit pack); this form costs 16 with packed fp32 instructions and 23 without
+// (the build turns them off, see the Makefile):
 //     a = min(|x|, 6)       e = exp2(-a^2 log2(e) / 2) = exp(-a^2 / 2)        q(a) = Phi(-a) exp(a^2 / 2) = erfcx(a / sqrt 2) / 2
 //     Phi(-a) = e q(a)      gelu(x) = max(x, 0) - a e q(a)                    gelu'(x) - 1/2 = copysign((a / sqrt(2 pi) - q(a)) e + 1/2, x)
 // ONE transcendental (v_exp_f32), no reciprocal: q is smooth and well conditioned on [0, 6] - a degree-8 minimax polynomial in a
 // holds it to 3.0e-4 RELATIVE (Lawson iteration on 6000 Chebyshev nodes, scripts/dev/gelu_fit.py), so Phi(-a) keeps its relative
 // accuracy down the tail where the A-S form (absolute error 1.5e-7) is 5e-3 off at x = -4 and 50 % at x = -5.  Everything but
-// min / max / exp / copysign is v_pk_{fma,mul}_f32 (two elements per issue slot).  (a/sqrt(2 pi) - q) e + 1/2 >= 0 for every a
+// min / max / exp / copysign is an fma or a product.  (a/sqrt(2 pi) - q) e + 1/2 >= 0 for every a
 // (it is 0 at a = 0 and rises), so one copysign carries the derivative's odd part.  Beyond |x| = 6 the tail term is frozen at
 // 6 Phi(-6) = 6e-9 (a is clamped: no overflow of the polynomial, never a NaN from a finite input).
 // Against fp64 erf-GELU on 2e6 points of [-8, 8] (tests/test_kernels_gpu.py::test_gelu_pair_dense_sweep): the bf16 result is within

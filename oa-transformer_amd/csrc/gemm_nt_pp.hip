@@ -111,8 +111,7 @@ OAT_DEV bool pp_epilogue(const GemmArgs& g, const f32x4 (&acc)[8][4], int m0, in
   float m8 = 0.f;
   uint32_t w8 = 0;                                     // the 4 quantised values of the last finish() call
   // EPI_GELU_GRAD: gelu / gelu' of a row group are formed COLUMN-wise before its rows are stored - an accumulator's four registers
-  // (rows r = 0..3 of one column) are two aligned register pairs, so the packed fp32 math of gelu_pair (common.h) runs on them in
-  // place; taken row-wise (four columns = four different accumulators) every packed operand would first be gathered by a v_mov.
+  // (rows r = 0..3 of one column) are two aligned register pairs, so gelu_pair (common.h) runs on them in place, two at a time.
   // Gc[j][r] = gelu, Hc[j][r] = the derivative: 8-bit code as a float (HU8: affine map applied, packed) or gelu' itself.
   f32x4 Gc[4], Hc[4];
   auto gelu_group = [&](int i) {
