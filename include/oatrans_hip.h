@@ -16,7 +16,7 @@
  *   - bf16 tensors are passed as `void*` (raw uint16 storage), fp32 as `float*`.
  *   - token-row layout used engine-wide: patch (b,f,n) -> row (b*T+f)*N+n ; CLS(b) -> row
  *     B*T*N+b  (M = B*T*N + B rows).  ld* arguments are row pitches in ELEMENTS.
- *   - head_dim is fixed at 64 (ViT-B/16 and DistilBERT-base).
+ *   - head_dim is fixed at 64 (ViT-B/16 and DistilBERT-base), but for the windowed attention (64 or 128).
  */
 #ifndef OATRANS_HIP_H
 #define OATRANS_HIP_H
@@ -285,6 +285,51 @@ int oat_attn_text_bwd(const void* qkv, int ldqkv, const void* mask, const void* 
                       const float* lse, float* delta_scratch, const void* dout, int lddo, void* dqkv,
                       int lddqkv, int B, int L, int H, int D, float scale, float drop_p, const void* rng,
                       unsigned drop_site, void* stream);
+/* ---- rotary positions and windowed attention (no counterpart in the reference: relative positions and local attention for token
+ * sequences beyond the divided space / time attention above - long clips as ONE sequence of (time, height, width) tokens with the
+ * class token as a sink, captions of any length, and text that is written token by token).
+ * dtype: 0 bf16, 1 fp16, 2 fp32 (oat_rope_axes only).  Pitches (ld*) and strides in ELEMENTS; rows and cache rows start on 16 bytes.
+ *
+ * Rotary positions: pair p of a head is turned by pos[row % period][axis[p]] * turns[p] whole turns (turns = frequency / 2 pi; the
+ * product is formed in 64 bits).  Pairs: (p, p + n_pairs), interleaved (2 p, 2 p + 1), of the head's first 2 * n_pairs values; the
+ * others pass through.  inverse: the turn back, which is also the gradient.  The struct is read on the host during the call. */
+typedef struct OatRope {
+  int n_pairs, n_axes, interleaved, reserved;      /* 1..64 pairs, 1..4 axes */
+  double turns[64];
+  unsigned char axis[64];
+} OatRope;
+/* x, out: [M, >= heads * dim], heads contiguous; out may be x (in place), no other overlap.  pos: int32 [period, n_axes], M a multiple of period. */
+int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dtype, const int* pos, int period, int M, int heads,
+                  int dim, const OatRope* rope, int inverse, void* stream);
+/* Attention over a sliding window with sinks, D = 64 or 128, query heads h sharing key head h / (Hq / Hkv).
+ * seqs: int32 [B, 4] on the device = (first query row, queries, first key row, keys) of every sequence - packed, padded or of different
+ * query and key counts; query i stands at p = i + keys - queries and sees key j if  j <= p + right  and  (j >= p - left or j < sinks);
+ * left / right < 0: no such edge (right = 0: causal).  A row that sees nothing gives 0 and lse = -inf.  Rows of no sequence are left as
+ * they were.  A sequence that does not fit rows_q / rows_k / max_q / max_k is taken as empty.  lse: fp32 [rows_q, Hq] (natural
+ * logarithm) or NULL.  Rows of a sequence have to be finite: what a masked pair holds is multiplied by an exact zero. */
+int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
+                        float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
+                        int left, int right, int sinks, float scale, void* stream);
+size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int Hq);
+/* dq, dk, dv of the same call (written, not accumulated; fixed order of every sum).  Sequences must not share query or key rows. */
+int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out, long long ldo,
+                        const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk, long long lddk, void* dv,
+                        long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
+                        int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* One new token of every sequence: qkv [B, (Hq + 2 Hkv) * D] (q | k | v); past[b] = tokens before it (< 0: takes no part: out is zero,
+ * the cache stays; so does a plain cache without a slot left).  The query and key are turned by pos [B, n_axes] (rope NULL: not), the key
+ * and value are written to their slot, and the query attends to what it sees.  Cache: cap slots; strides = 6 element strides {k: sequence, slot,
+ * head; v: the same}, D contiguous.  Plain: token t in slot t, window `left` (< 0: none) and sinks as above.  Rolling: cap = sinks + left + 1
+ * slots, slot(t) = t < sinks ? t : sinks + (t - sinks) % (cap - sinks).  One launch.  workspace: zero before the first use, left ready
+ * for the next call; calls that may run at the same time need one each. */
+size_t oat_attn_window_step_workspace_bytes(int B, int Hq, int Hkv, int D);
+int oat_attn_window_step(const void* qkv, long long ldqkv, const int* past, void* k_cache, void* v_cache, const long long* strides, int cap,
+                         void* out, long long ldo, int B, int Hq, int Hkv, int D, int dtype, int left, int sinks, int rolling, float scale,
+                         const OatRope* rope, const int* pos, void* workspace, size_t workspace_bytes, void* stream);
+/* A prompt's (turned) keys and values into a cache: slots as above; a prompt of more than cap tokens leaves its sinks and its last ones. */
+int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k, int max_k,
+                          void* k_cache, void* v_cache, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream);
+
 /* ---- input pipeline, device side: decoded frames -> clip tensor.  Replaces, per batch and in one launch,
  * frames.float() / 255 (base/base_dataset.py:519,533,544) and the tensor transforms of data_loader/transforms.py:4-31 /
  * base_dataset_global_local.py:251-257: crop box + bilinear resize (= torchvision Resize on tensors =

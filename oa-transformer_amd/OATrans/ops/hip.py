@@ -30,6 +30,23 @@ def declared_symbols():
     return sorted(set(re.findall(r"\b(oat_[a-z0-9_]+)\s*\(", text)))
 
 
+class _OatRope(ctypes.Structure):
+    _fields_ = [("n_pairs", ctypes.c_int), ("n_axes", ctypes.c_int), ("interleaved", ctypes.c_int), ("reserved", ctypes.c_int),
+                ("turns", ctypes.c_double * 64), ("axis", ctypes.c_ubyte * 64)]
+
+
+_P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
+_WINDOW_SIGNATURES = {
+    "oat_rope_axes": (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _I, _I, ctypes.POINTER(_OatRope), _I, _P]),
+    "oat_attn_window_fwd": (_I, [_P, _L] * 4 + [_P, _P] + [_I] * 12 + [_F, _P]),
+    "oat_attn_window_bwd_workspace_bytes": (_Z, [_I, _I]),
+    "oat_attn_window_bwd": (_I, [_P, _L] * 4 + [_P] + [_P, _L] * 4 + [_P] + [_I] * 12 + [_F, _P, _Z, _P]),
+    "oat_attn_window_step_workspace_bytes": (_Z, [_I] * 4),
+    "oat_attn_window_step": (_I, [_P, _L, _P, _P, _P, ctypes.POINTER(_L), _I, _P, _L] + [_I] * 8 + [_F, ctypes.POINTER(_OatRope), _P, _P, _Z, _P]),
+    "oat_window_cache_fill": (_I, [_P, _L, _P, _L, _P, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _I, _I, _I, _P]),
+}
+
+
 def lib():
     global _lib
     if _lib is None:
@@ -42,6 +59,8 @@ def lib():
         _lib.oat_tn_group_slab_bytes.restype = ctypes.c_size_t
         _lib.oat_infonce_workspace_floats.restype = ctypes.c_size_t
         _lib.oat_sim_workspace_floats.restype = ctypes.c_size_t
+        for name, (res, args) in _WINDOW_SIGNATURES.items():
+            getattr(_lib, name).restype, getattr(_lib, name).argtypes = res, args
         for name in declared_symbols():
             if not hasattr(_lib, name):
                 raise OatError(f"liboatrans_hip.so lacks symbol {name}")
@@ -961,3 +980,224 @@ def patch_masks(bbox, P=14, box_class=None, sel_class=None):
     _check(lib().oat_patch_masks(_ptr(bbox), ldb, _ptr(box_class), _ptr(sel_class), _ptr(out), B, NB, O, P, _stream()),
            "oat_patch_masks")
     return out
+
+
+# ----------------------------------------------------------------------------- rotary positions and windowed attention
+_ELEMENTS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class RopeAxes:
+    """The ladder of a rotary position embedding over 1 to 4 axes, e.g. (time, height, width).
+
+    sections: rotated values of a head per axis (even numbers, in this order; what is left of the head passes through).
+    theta: pair i of n has frequency theta^(-i / n) - counted within its own axis, or (shared) over all pairs of the head.
+    interleaved: pairs are neighbours (2 p, 2 p + 1) instead of (p, p + half of the rotated values)."""
+
+    def __init__(self, sections, theta=10000.0, interleaved=False, shared=False):
+        import math
+        sections = [int(d) for d in sections]
+        if not 1 <= len(sections) <= 4 or any(d < 0 or d % 2 for d in sections) or not 2 <= sum(sections) <= 128:
+            raise OatError("RopeAxes: 1 to 4 axes of an even number of values, 2 to 128 in all")
+        if not (float(theta) > 0.0 and math.isfinite(theta)):
+            raise OatError("RopeAxes: theta must be a positive number")
+        self.sections, self.theta, self.interleaved, self.shared = tuple(sections), float(theta), bool(interleaved), bool(shared)
+        self.axes, self.pairs = len(sections), sum(sections) // 2
+        self.struct = _OatRope(n_pairs=self.pairs, n_axes=self.axes, interleaved=int(self.interleaved))
+        p = 0
+        for a, d in enumerate(sections):
+            for i in range(d // 2):
+                exponent = -2.0 * p / sum(sections) if shared else -2.0 * i / d
+                self.struct.axis[p], self.struct.turns[p] = a, self.theta ** exponent / (2.0 * math.pi)
+                p += 1
+
+    def frequencies(self):
+        """fp64 [pairs] radians per position, int64 [pairs] axis (host)."""
+        import math
+        n = self.pairs
+        return (torch.tensor([self.struct.turns[p] * 2.0 * math.pi for p in range(n)], dtype=torch.float64),
+                torch.tensor([self.struct.axis[p] for p in range(n)]))
+
+
+def _need(ok, why):
+    if not ok:
+        raise OatError(why)
+
+
+def _launch(device, call, what):
+    """call(stream) on the current stream of `device`, which need not be the current device."""
+    if device.type != "cuda":
+        raise OatError(f"{what} runs on MI355X only (no CPU path)")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = call(torch.cuda.current_stream().cuda_stream)
+    else:
+        rc = call(torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        _check(rc, what)
+
+
+def _rows(t, columns, dtype, device, what):
+    """t is a [rows, >= columns] matrix of dtype with neighbouring columns"""
+    if t.dim() != 2 or t.shape[1] < columns or (t.stride(1) != 1 and t.shape[1] > 1) or t.dtype != dtype or t.device != device:
+        raise OatError(f"{what}: need [rows, {columns}] of {dtype} on {device} with unit column stride, got {list(t.shape)} {t.dtype} "
+                       f"on {t.device}, strides {t.stride()}")
+
+
+def _ld(t):
+    # (a matrix of one row may carry any row stride, and never uses it)
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rope_axes(x, pos, rope, heads, head_dim, out=None, inverse=False):
+    """Rotary positions on x [M, heads * head_dim] (bf16 / fp16 / fp32; a column slice of packed q | k | v rows will do).
+    pos: int32 [P, axes], M a multiple of P: row m stands at pos[m % P].  out: where to (x itself: in place; default: a new
+    tensor).  inverse: the turn back = the gradient's way."""
+    _need(x.dtype in _ELEMENTS, "rope_axes: x must be bf16, fp16 or fp32")
+    _rows(x, heads * head_dim, x.dtype, x.device, "rope_axes: x")
+    _need(pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape[1] == rope.axes and pos.is_contiguous() and pos.device == x.device,
+          f"rope_axes: pos must be a contiguous int32 [P, {rope.axes}] on {x.device}")
+    M = x.shape[0]
+    if out is None:
+        out = torch.empty(M, heads * head_dim, dtype=x.dtype, device=x.device)
+    else:
+        _rows(out, heads * head_dim, x.dtype, x.device, "rope_axes: out")
+        _need(out.shape[0] == M, "rope_axes: out has another number of rows")
+    _launch(x.device, lambda s: lib().oat_rope_axes(x.data_ptr(), _ld(x), out.data_ptr(), _ld(out), _ELEMENTS[x.dtype], pos.data_ptr(),
+                                                    pos.shape[0], M, heads, head_dim, rope.struct, int(inverse), s), "oat_rope_axes")
+    return out
+
+
+def seq_table(q_lens, k_lens=None, q_rows=None, k_rows=None, device="cuda"):
+    """int32 [B, 4] = (first query row, queries, first key row, keys) for the windowed attention, from host counts.
+    q_rows / k_rows: first rows (default: packed one after the other; a padded batch of length L: range(0, B * L, L))."""
+    q_lens = [int(n) for n in q_lens]
+    k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+    _need(len(k_lens) == len(q_lens) and all(0 <= n < 2 ** 29 for n in q_lens + k_lens), "seq_table: one count of 0 to 2^29 per sequence")
+
+    def starts(lens, rows):
+        if rows is not None:
+            return [int(r) for r in rows]
+        out, at = [], 0
+        for n in lens:
+            out.append(at)
+            at += n
+        return out
+    q_rows, k_rows = starts(q_lens, q_rows), starts(k_lens, q_rows if k_rows is None and k_lens is q_lens else k_rows)
+    _need(len(q_rows) == len(k_rows) == len(q_lens), "seq_table: one first row per sequence")
+    return torch.tensor(list(zip(q_rows, q_lens, k_rows, k_lens)), dtype=torch.int32).reshape(-1, 4).to(device)
+
+
+def _window_args(q, k, v, seqs, heads, kv_heads, D, what):
+    _need(q.dtype in (torch.bfloat16, torch.float16), f"{what}: q, k, v must be bf16 or fp16")
+    _rows(q, heads * D, q.dtype, q.device, f"{what}: q")
+    _rows(k, kv_heads * D, q.dtype, q.device, f"{what}: k")
+    _rows(v, kv_heads * D, q.dtype, q.device, f"{what}: v")
+    _need(k.shape[0] == v.shape[0], f"{what}: k and v have different numbers of rows")
+    _need(seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[1] == 4 and seqs.is_contiguous() and seqs.device == q.device,
+          f"{what}: seqs must be a contiguous int32 [B, 4] on {q.device}")
+
+
+def attn_window_fwd(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, left=-1, right=0, sinks=0, scale=None, out=None, lse=None):
+    """out [rows, heads * head_dim] = attention of q over k, v within a sliding window with sinks (see oat_attn_window_fwd).
+    seqs: int32 [B, 4] on the device (seq_table); max_q / max_k: the largest counts in it.  lse: fp32 [rows, heads], written where
+    given (the backward pass needs it).  A new `out` starts as zeros, a given one keeps its rows of no sequence."""
+    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, "attn_window_fwd")
+    if out is None:
+        out = torch.zeros(q.shape[0], heads * head_dim, dtype=q.dtype, device=q.device)
+    _rows(out, heads * head_dim, q.dtype, q.device, "attn_window_fwd: out")
+    _need(out.shape[0] == q.shape[0], "attn_window_fwd: out has another number of rows than q")
+    _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (q.shape[0], heads) and lse.is_contiguous() and lse.device == q.device),
+          "attn_window_fwd: lse must be a contiguous fp32 [rows, heads]")
+    _launch(q.device, lambda s: lib().oat_attn_window_fwd(
+        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr() if lse is not None else None,
+        seqs.data_ptr(), seqs.shape[0], max_q, max_k, q.shape[0], k.shape[0], heads, kv_heads, head_dim, _ELEMENTS[q.dtype], left, right,
+        sinks, head_dim ** -0.5 if scale is None else scale, s), "oat_attn_window_fwd")
+    return out
+
+
+def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, max_q, max_k, left=-1, right=0, sinks=0, scale=None,
+                    dq=None, dk=None, dv=None, workspace=None):
+    """(dq, dk, dv) of attn_window_fwd.  New outputs start as zeros, given ones keep their rows of no sequence.  workspace: fp32 of
+    oat_attn_window_bwd_workspace_bytes(rows, heads) bytes (default: a new one)."""
+    what = "attn_window_bwd"
+    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, what)
+    D, dt, dev, M = head_dim, q.dtype, q.device, q.shape[0]
+    _rows(out, heads * D, dt, dev, what + ": out")
+    _rows(dout, heads * D, dt, dev, what + ": dout")
+    _need(out.shape[0] == dout.shape[0] == M, what + ": out and dout have as many rows as q")
+    _need(lse.dtype == torch.float32 and lse.shape == (M, heads) and lse.is_contiguous() and lse.device == dev,
+          what + ": lse must be a contiguous fp32 [rows, heads]")
+    dq = torch.zeros(M, heads * D, dtype=dt, device=dev) if dq is None else dq
+    dk = torch.zeros(k.shape[0], kv_heads * D, dtype=dt, device=dev) if dk is None else dk
+    dv = torch.zeros(k.shape[0], kv_heads * D, dtype=dt, device=dev) if dv is None else dv
+    _rows(dq, heads * D, dt, dev, what + ": dq")
+    _rows(dk, kv_heads * D, dt, dev, what + ": dk")
+    _rows(dv, kv_heads * D, dt, dev, what + ": dv")
+    _need(dq.shape[0] == M and dk.shape[0] == dv.shape[0] == k.shape[0], what + ": dq, dk, dv have as many rows as q, k, v")
+    if workspace is None:
+        workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, heads) // 4, dtype=torch.float32, device=dev)
+    _need(workspace.is_contiguous() and workspace.device == dev, what + ": workspace must be contiguous on the same device")
+    _launch(dev, lambda s: lib().oat_attn_window_bwd(
+        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr(), dout.data_ptr(), _ld(dout),
+        dq.data_ptr(), _ld(dq), dk.data_ptr(), _ld(dk), dv.data_ptr(), _ld(dv), seqs.data_ptr(), seqs.shape[0], max_q, max_k, M, k.shape[0],
+        heads, kv_heads, D, _ELEMENTS[dt], left, right, sinks, D ** -0.5 if scale is None else scale, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), s), "oat_attn_window_bwd")
+    return dq, dk, dv
+
+
+def _cache_args(k_cache, v_cache, what):
+    ok = (k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.device == v_cache.device
+          and k_cache.dtype in (torch.bfloat16, torch.float16) and k_cache.stride(3) == v_cache.stride(3) == 1)
+    if not ok:
+        raise OatError(f"{what}: the caches must be [B, slots, heads, head_dim] of bf16 or fp16, both alike, with unit last stride")
+    return (_L * 6)(*k_cache.stride()[:3], *v_cache.stride()[:3])
+
+
+def window_step_workspace(B, heads, kv_heads, head_dim, device="cuda"):
+    """The zeroed workspace of attn_window_step (its contents belong to the operator; steps that may run at once need one each)."""
+    return torch.zeros(lib().oat_attn_window_step_workspace_bytes(B, heads, kv_heads, head_dim) // 4, dtype=torch.float32, device=device)
+
+
+def attn_window_step(qkv, past, k_cache, v_cache, heads, left=-1, sinks=0, rolling=False, scale=None, rope=None, pos=None, pieces=None,
+                     out=None):
+    """One new token of every sequence against its cache (see oat_attn_window_step): qkv [B, (heads + 2 * kv_heads) * head_dim], past
+    int32 [B] tokens so far (< 0: takes no part), caches [B, slots, kv_heads, head_dim] (written: the new key and value).
+    rope / pos int32 [B, axes]: turn query and key.  pieces: window_step_workspace(...) (default: a new one)."""
+    what = "attn_window_step"
+    strides = _cache_args(k_cache, v_cache, what)
+    B, cap, kv_heads, D = k_cache.shape
+    dev, dt = qkv.device, qkv.dtype
+    _need(dt == k_cache.dtype and dev == k_cache.device, what + ": qkv and the caches differ in type or device")
+    _rows(qkv, (heads + 2 * kv_heads) * D, dt, dev, what + ": qkv")
+    _need(qkv.shape[0] == B, what + ": one row of qkv per sequence")
+    _need(past.dtype == torch.int32 and past.shape == (B,) and past.is_contiguous() and past.device == dev, what + ": past must be int32 [B]")
+    _need(rope is None or (pos is not None and pos.dtype == torch.int32 and pos.shape == (B, rope.axes) and pos.is_contiguous() and pos.device == dev),
+          what + ": pos must be a contiguous int32 [B, axes]")
+    if pieces is None:
+        pieces = window_step_workspace(B, heads, kv_heads, D, dev)
+    _need(pieces.is_contiguous() and pieces.device == dev, what + ": pieces must be contiguous on the same device")
+    if out is None:
+        out = torch.empty(B, heads * D, dtype=dt, device=dev)
+    else:
+        _rows(out, heads * D, dt, dev, what + ": out")
+        _need(out.shape[0] == B, what + ": one row of out per sequence")
+    _launch(dev, lambda s: lib().oat_attn_window_step(
+        qkv.data_ptr(), _ld(qkv), past.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, cap, out.data_ptr(), _ld(out), B, heads,
+        kv_heads, D, _ELEMENTS[dt], left, sinks, int(rolling), D ** -0.5 if scale is None else scale,
+        rope.struct if rope is not None else None, pos.data_ptr() if rope is not None else None, pieces.data_ptr(),
+        pieces.numel() * pieces.element_size(), s), "oat_attn_window_step")
+    return out
+
+
+def window_cache_fill(k, v, seqs, k_cache, v_cache, max_k, sinks=0):
+    """A prompt's keys and values (rows of seqs) into the caches; more tokens than slots: the sinks and the last ones stay."""
+    what = "window_cache_fill"
+    strides = _cache_args(k_cache, v_cache, what)
+    B, cap, kv_heads, D = k_cache.shape
+    _rows(k, kv_heads * D, k_cache.dtype, k_cache.device, what + ": k")
+    _rows(v, kv_heads * D, k_cache.dtype, k_cache.device, what + ": v")
+    _need(k.shape[0] == v.shape[0], what + ": k and v have different numbers of rows")
+    _need(seqs.dtype == torch.int32 and seqs.shape == (B, 4) and seqs.is_contiguous() and seqs.device == k.device, what + ": seqs must be int32 [B, 4]")
+    _launch(k.device, lambda s: lib().oat_window_cache_fill(
+        k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), seqs.data_ptr(), B, k.shape[0], max_k, k_cache.data_ptr(), v_cache.data_ptr(), strides,
+        cap, kv_heads, D, sinks, s), "oat_window_cache_fill")

@@ -1,0 +1,135 @@
+// Tiles, fragments and visibility shared by the windowed-attention kernels (attn_window.hip: forward and backward).
+//
+// Matrix instruction 32x32x16 (16-bit operands, fp32 sums):
+//   A: lane l holds A[row = l & 31][k = (l >> 5) * 8 .. +8]     B: lane l holds B[k = (l >> 5) * 8 .. +8][col = l & 31]
+//   C: lane l, register r holds C[row = 8 * (r >> 2) + 4 * (l >> 5) + (r & 3)][col = l & 31]
+// A product's C can be the next product's B without leaving the registers, because the order of a sum's terms is free: registers
+// 8c .. 8c + 7 of a lane are the rows 16 c + 8 * (e >> 2) + 4 * (l >> 5) + (e & 3), e = 0..7, and the A fragments of that next
+// product are read from the LDS (transposing reads) in the same order of k.
+#pragma once
+#include "rope.h"
+#include <stdio.h>
+
+namespace oat {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+template <class T> OAT_DEV f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c);
+template <> OAT_DEV f32x16 mfma32<bf16>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> OAT_DEV f32x16 mfma32<_Float16>(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// registers 8c .. 8c + 7 as a B fragment: one rounding of each value to the operands' type (the matrix unit takes no 32-bit operand
+// at this rate); the sums stay in 32 bits
+template <class T> OAT_DEV s16x8 pack8(const f32x16& x, int c) {
+  typedef __attribute__((ext_vector_type(8))) T T8;
+  T8 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = (T)x[8 * c + e];
+  return __builtin_bit_cast(s16x8, y);
+}
+
+// ---- tiles of 64 rows in the LDS, rows of D 16-bit values in chunks of 16 bytes.  Chunk c of row r stands at place c ^ swz(r): a row
+// fragment (16 rows, one chunk) and a transposing read (4 rows of 4 neighbouring chunks, or 8 of 2) then touch every bank alike.
+template <int D> OAT_DEV int swz(int r) { return (D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2) | ((r >> 2) & 1) << 1 | ((r >> 3) & 1); }
+
+constexpr int TILE = 64;
+
+// asynchronous copy of a tile by 256 threads: rows 0 .. TILE - 1 from `base` (wave-uniform), pitch `ldb` bytes; rows past `last`
+// repeat that row, so that no memory outside the sequence is read and nothing but its own finite values stands in the tile
+template <int D> OAT_DEV void stage_tile(const char* base, uint32_t ldb, int last, uint32_t lds) {
+  constexpr int CPR = D / 8;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+  for (int i = 0; i < TILE * CPR / 256; ++i) {
+    const int c = i * 256 + tid, r = c / CPR, ch = (c % CPR) ^ swz<D>(r);
+    glds16_asm_lds(base, (uint32_t)min(r, last) * ldb + ch * 16, lds + (i * 256 + wave * 64) * 16);
+  }
+}
+// A fragment: rows rb .. rb + 31 of a tile, k = 16 ks .. +16
+template <int D> OAT_DEV s16x8 row_frag32(const char* tile, int rb, int ks) {
+  const int lane = threadIdx.x & 63, r = lane & 31;
+  return *reinterpret_cast<const s16x8*>(tile + (rb + r) * (D * 2) + (((2 * ks + (lane >> 5)) ^ swz<D>(r)) << 4));
+}
+// A fragment of the transposed tile: rows d = 32 dt .. +32, k = the tile's rows kb .. kb + 15 in the order of a C fragment's registers
+template <int D> OAT_DEV s16x8 col_frag32(const char* tile, int kb, int dt) {
+  const int lane = threadIdx.x & 63, j = (lane >> 2) & 3, q4 = lane & 3;
+  const int ch = dt * 4 + ((lane >> 4) & 1) * 2 + (q4 >> 1);
+  s16x8 out;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = 8 * e + 4 * (lane >> 5) + j;
+    const s16x4 h = lds_tr16(tile + (kb + r) * (D * 2) + ((ch ^ swz<D>(r)) << 4) + (q4 & 1) * 8);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) out[4 * e + x] = h[x];
+  }
+  return out;
+}
+// B fragments of 32 rows in memory (row = the lane's column of the product)
+template <int D> OAT_DEV void load_cols(s16x8 (&f)[D / 16], const char* row) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) f[ks] = *reinterpret_cast<const s16x8*>(row + (2 * ks + half) * 16);
+}
+OAT_DEV float both_halves(float v, bool max) {
+  const float o = __shfl_xor(v, 32, 64);
+  return max ? fmaxf(v, o) : v + o;
+}
+// every wave's copies have landed and every wave is done reading what the next copies overwrite
+OAT_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ---- sequences and visibility.  Query i of a sequence stands at position p = i + nk - nq (its last query at its last key); it sees
+// key j if  j <= p + right  and  (j >= p - left  or  j < sinks).
+struct WinArgs {
+  const char *q, *k, *v, *o, *dout;
+  char *out, *dq, *dk, *dv;
+  float* lse;                           // [rows_q, Hq], natural logarithm; -inf: the row sees nothing
+  float *lse2, *delta;                  // backward: [Hq, rows_q], base 2; sum of dout * out
+  long long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;      // bytes
+  const int4* seqs;                     // first query row, queries, first key row, keys
+  int B, Hq, Hkv, left, right, sinks, max_q, max_k, rows_q, rows_k;
+  float scale;
+};
+struct Seq { int q0, nq, k0, nk; };
+// a sequence that does not fit the buffers (or the launch) is taken as empty: nothing outside is read or written
+OAT_DEV Seq load_seq(const WinArgs& a, int b) {
+  const int4 s = a.seqs[b];
+  const bool ok = s.x >= 0 && s.y >= 0 && s.z >= 0 && s.w >= 0 && s.y <= a.max_q && s.w <= a.max_k && (long long)s.x + s.y <= a.rows_q &&
+                  (long long)s.z + s.w <= a.rows_k;
+  return ok ? Seq{s.x, s.y, s.z, s.w} : Seq{0, 0, 0, 0};
+}
+// blockIdx -> (tile, head, sequence).  Workgroups go to the 8 XCDs in turn: each XCD gets a contiguous share of the (sequence, head,
+// tile) list, so the tiles of one head and the heads that share keys meet in one L2.
+struct Place { int b, h, tile; };
+OAT_DEV bool place(int tiles, int heads, int B, Place& p) {
+  const int per = gridDim.x >> 3;
+  const int i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (i >= tiles * heads * B) return false;
+  p.tile = i % tiles;
+  p.h = i / tiles % heads;
+  p.b = i / tiles / heads;
+  return true;
+}
+inline unsigned place_grid(long long n) { return (unsigned)((n + 7) / 8 * 8); }
+
+// the key tiles (of 64) that queries at positions p0 .. p1 see: those of the sinks, then those of the window
+struct KeyTiles {
+  int sink, first, count;
+  OAT_DEV int at(int n) const { return n < sink ? n : first + n - sink; }
+};
+OAT_DEV KeyTiles key_tiles(const WinArgs& a, int nk, int p0, int p1) {
+  const int hi = min(nk - 1, p1 + a.right);
+  if (hi < 0) return {0, 0, 0};
+  const int end = hi / TILE + 1;
+  const int sink = min((min(a.sinks, nk) + TILE - 1) / TILE, end);
+  const int first = max(max(0, p0 - a.left) / TILE, sink);
+  return {sink, first, sink + max(0, end - first)};
+}
+
+}  // namespace oat

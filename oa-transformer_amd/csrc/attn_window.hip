@@ -1,0 +1,434 @@
+// Attention over a sliding window with sinks: forward and backward, ragged sequences, shared key heads.
+#include "attn_window.h"
+
+namespace oat {
+
+// ---------------------------------------------------------------------------------------------- forward
+// One workgroup = 128 queries of one head, a wave = 32 of them; keys and values pass through the LDS in tiles of 64.
+//     S^T = K Q^T      P^T = exp2(c S^T - c m)      O^T += V^T P^T       c = scale log2(e), m = running maximum of the row
+// The query is the COLUMN of S^T: a lane holds 16 of 32 keys of ONE query, so maximum and sum of a row are register work and one
+// exchange with lane ^ 32, and P^T is the B operand of the second product where it stands.
+template <class T, int D>
+__global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
+  constexpr int TB = TILE * D * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TB];         // K, V x 2
+  const int tiles = (a.max_q + 127) / 128;
+  Place pl;
+  if (!place(tiles, a.Hq, a.B, pl)) return;
+  const Seq s = load_seq(a, pl.b);
+  const int i0 = (tiles - 1 - pl.tile) * 128;                          // causal rows are longest at the end: those first
+  if (i0 >= s.nq) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int off = s.nk - s.nq, hk = pl.h / (a.Hq / a.Hkv);
+  const KeyTiles kt = key_tiles(a, s.nk, i0 + off, min(i0 + 127, s.nq - 1) + off);
+  const char* kb = a.k + (long long)s.k0 * a.ldk + hk * (D * 2);
+  const char* vb = a.v + (long long)s.k0 * a.ldv + hk * (D * 2);
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
+  auto stage = [&](int n) {
+    const int j0 = kt.at(n) * TILE;
+    stage_tile<D>(kb + (long long)j0 * a.ldk, (uint32_t)a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
+    stage_tile<D>(vb + (long long)j0 * a.ldv, (uint32_t)a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
+  };
+  const int iw = i0 + wave * 32, i = iw + (lane & 31), ic = min(i, s.nq - 1);
+  const int p = ic + off, hi = min(s.nk - 1, p + a.right), lo = p - a.left;
+  const int wp0 = iw + off, wp1 = min(iw + 31, s.nq - 1) + off;
+  const float c = a.scale * LOG2E;
+  s16x8 qf[D / 16];
+  load_cols<D>(qf, a.q + (long long)(s.q0 + ic) * a.ldq + pl.h * (D * 2));
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (kt.count) stage(0);
+  for (int n = 0; n < kt.count; ++n) {
+    tile_barrier();
+    if (n + 1 < kt.count) stage(n + 1);
+    const int j0 = kt.at(n) * TILE;
+    if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) continue;
+    const bool full = j0 + TILE - 1 <= min(s.nk - 1, wp0 + a.right) && (j0 >= wp1 - a.left || j0 + TILE - 1 < a.sinks);
+    const char* Kt = lds + (n & 1) * 2 * TB;
+    const char* Vt = Kt + TB;
+    f32x16 st[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[u][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) st[u] = mfma32<T>(row_frag32<D>(Kt, u * 32, ks), qf[ks], st[u]);
+    }
+    if (!full) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + u * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (!(j <= hi && (j >= lo || j < a.sinks))) st[u][r] = -INFINITY;
+        }
+    }
+    float mx = st[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[u][r]);
+    const float mn = fmaxf(m, both_halves(mx, true));
+    const float mc = mn == -INFINITY ? 0.f : mn * c;
+    if (__any(mn > m)) {
+      const float al = __builtin_amdgcn_exp2f(m * c - mc);
+      l *= al;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= al;
+      m = mn;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        st[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[u][r], c, -mc));
+        l += st[u][r];
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const s16x8 pf = pack8<T>(st[u], h);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma32<T>(col_frag32<D>(Vt, u * 32 + h * 16, dt), pf, o[dt]);
+      }
+  }
+  if (i >= s.nq) return;
+  l = both_halves(l, false);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  char* po = a.out + (long long)(s.q0 + i) * a.ldo + pl.h * (D * 2);
+  typedef __attribute__((ext_vector_type(4))) T T4;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      T4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)(o[dt][4 * g + e] * inv);
+      *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = y;
+    }
+  if (a.lse && half == 0) a.lse[(size_t)(s.q0 + i) * a.Hq + pl.h] = l > 0.f ? m * a.scale + __logf(l) : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------- backward
+// With P from the saved log-sum-exp and delta_i = sum_d dO_id O_id:
+//     dV_j = sum_i P_ij dO_i     dS_ij = P_ij (dO_i . V_j - delta_i)     dQ_i = scale sum_j dS_ij K_j     dK_j = scale sum_i dS_ij Q_i
+// Two kernels that form S and dO V^T again, one over queries (dQ), one over keys (dK, dV; the query heads that share a key head are
+// summed in the workgroup): 7 products for the 5 of one kernel with atomic sums, but every sum has one fixed order.
+
+// dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
+template <class T, int D>
+__global__ __launch_bounds__(256) void win_bwd_q_kernel(WinArgs a) {
+  constexpr int TB = TILE * D * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
+  const int tiles = (a.max_q + 127) / 128;
+  Place pl;
+  if (!place(tiles, a.Hq, a.B, pl)) return;
+  const Seq s = load_seq(a, pl.b);
+  const int i0 = (tiles - 1 - pl.tile) * 128;
+  if (i0 >= s.nq) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int off = s.nk - s.nq, hk = pl.h / (a.Hq / a.Hkv);
+  const KeyTiles kt = key_tiles(a, s.nk, i0 + off, min(i0 + 127, s.nq - 1) + off);
+  const char* kb = a.k + (long long)s.k0 * a.ldk + hk * (D * 2);
+  const char* vb = a.v + (long long)s.k0 * a.ldv + hk * (D * 2);
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
+  auto stage = [&](int n) {
+    const int j0 = kt.at(n) * TILE;
+    stage_tile<D>(kb + (long long)j0 * a.ldk, (uint32_t)a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
+    stage_tile<D>(vb + (long long)j0 * a.ldv, (uint32_t)a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
+  };
+  const int iw = i0 + wave * 32, i = iw + (lane & 31), ic = min(i, s.nq - 1);
+  const int p = ic + off, hi = min(s.nk - 1, p + a.right), lo = p - a.left;
+  const int wp0 = iw + off, wp1 = min(iw + 31, s.nq - 1) + off;
+  const float c = a.scale * LOG2E;
+  const long long row = s.q0 + ic;
+  s16x8 qf[D / 16], df[D / 16];
+  load_cols<D>(qf, a.q + row * a.ldq + pl.h * (D * 2));
+  load_cols<D>(df, a.dout + row * a.lddo + pl.h * (D * 2));
+  float delta = 0.f;
+  {
+    s16x8 of[D / 16];
+    load_cols<D>(of, a.o + row * a.ldo + pl.h * (D * 2));
+    typedef __attribute__((ext_vector_type(8))) T T8;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const T8 x = __builtin_bit_cast(T8, df[ks]), y = __builtin_bit_cast(T8, of[ks]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta += (float)x[e] * (float)y[e];
+    }
+    delta = both_halves(delta, false);
+  }
+  float lse2 = a.lse[(size_t)row * a.Hq + pl.h] * LOG2E;
+  if (!(lse2 > -INFINITY)) lse2 = 0.f;                                 // a row that sees nothing: every pair of it is masked below
+  if (i < s.nq && half == 0) {
+    a.lse2[(size_t)pl.h * a.rows_q + row] = lse2;
+    a.delta[(size_t)pl.h * a.rows_q + row] = delta;
+  }
+  f32x16 dq[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[dt][r] = 0.f;
+  if (kt.count) stage(0);
+  for (int n = 0; n < kt.count; ++n) {
+    tile_barrier();
+    if (n + 1 < kt.count) stage(n + 1);
+    const int j0 = kt.at(n) * TILE;
+    if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) continue;
+    const bool full = j0 + TILE - 1 <= min(s.nk - 1, wp0 + a.right) && (j0 >= wp1 - a.left || j0 + TILE - 1 < a.sinks);
+    const char* Kt = lds + (n & 1) * 2 * TB;
+    const char* Vt = Kt + TB;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        st = mfma32<T>(row_frag32<D>(Kt, u * 32, ks), qf[ks], st);
+        dp = mfma32<T>(row_frag32<D>(Vt, u * 32, ks), df[ks], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -lse2));
+        st[r] = pr * (dp[r] - delta);
+      }
+      if (!full) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + u * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (!(j <= hi && (j >= lo || j < a.sinks))) st[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const s16x8 sf = pack8<T>(st, h);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma32<T>(col_frag32<D>(Kt, u * 32 + h * 16, dt), sf, dq[dt]);
+      }
+    }
+  }
+  if (i >= s.nq) return;
+  char* po = a.dq + row * a.lddq + pl.h * (D * 2);
+  typedef __attribute__((ext_vector_type(4))) T T4;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      T4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)(dq[dt][4 * g + e] * a.scale);
+      *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = y;
+    }
+}
+
+// dK and dV of 128 keys (32 a wave): S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and
+// their gradients pass through the LDS in tiles of 64, with their lse2 and delta
+template <class T, int D>
+__global__ __launch_bounds__(256) void win_bwd_kv_kernel(WinArgs a) {
+  constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * ST];
+  const int tiles = (a.max_k + 127) / 128;
+  Place pl;
+  if (!place(tiles, a.Hkv, a.B, pl)) return;
+  const Seq s = load_seq(a, pl.b);
+  const int j0 = pl.tile * 128;
+  if (j0 >= s.nk) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int off = s.nk - s.nq, G = a.Hq / a.Hkv;
+  // queries that see any of these keys
+  auto first_q = [&](int j) { return max(0, j - a.right - off); };
+  auto last_q = [&](int jl, int jh) { return jl < a.sinks ? s.nq - 1 : min(s.nq - 1, jh + a.left - off); };
+  const int jend = min(j0 + 127, s.nk - 1);
+  const int t0 = first_q(j0) / TILE, t1 = last_q(j0, jend) < first_q(j0) ? t0 - 1 : last_q(j0, jend) / TILE;
+  const int nt = max(0, t1 - t0 + 1), count = nt * G;
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
+  auto stage = [&](int n) {
+    const int g = n / nt, i0 = (t0 + n - g * nt) * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
+    const long long row = s.q0 + i0;
+    const uint32_t l = l0 + (n & 1) * ST;
+    stage_tile<D>(a.q + row * a.ldq + h * (D * 2), (uint32_t)a.ldq, last, l);
+    stage_tile<D>(a.dout + row * a.lddo + h * (D * 2), (uint32_t)a.lddo, last, l + TB);
+    if (wave < 2) {
+      const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
+      const uint32_t dst = l + 2 * TB + wave * 256;
+      uint32_t keep;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                   : "=&s"(keep) : "v"((uint32_t)min(lane, last) * 4u), "s"(src), "s"(dst) : "memory");
+    }
+  };
+  const int jw = j0 + wave * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1);
+  const int jwe = min(jw + 31, s.nk - 1);
+  const float c = a.scale * LOG2E;
+  s16x8 kf[D / 16], vf[D / 16];
+  load_cols<D>(kf, a.k + (long long)(s.k0 + jc) * a.ldk + pl.h * (D * 2));
+  load_cols<D>(vf, a.v + (long long)(s.k0 + jc) * a.ldv + pl.h * (D * 2));
+  const int ilo = j - a.right - off, ihi = j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off);   // this key's queries
+  const int wlo = first_q(jw), whi = last_q(jw, jwe);                                                  // those of any key of the wave
+  const int flo = jwe - a.right - off, fhi = jwe < a.sinks ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);   // those of every key
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
+  if (count) stage(0);
+  for (int n = 0; n < count; ++n) {
+    tile_barrier();
+    if (n + 1 < count) stage(n + 1);
+    const int it = (t0 + n % nt) * TILE;
+    const char* Qt = lds + (n & 1) * ST;
+    const char* Dt = Qt + TB;
+    const float* Lt = reinterpret_cast<const float*>(Dt + TB);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int iu = it + u * 32;
+      if (jw >= s.nk || iu > whi || iu + 31 < wlo) continue;
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
+        dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(Lt + u * 32 + 8 * g + 4 * half);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(Lt + 64 + u * 32 + 8 * g + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -ls[e]));
+          dp[r] -= de[e];
+        }
+      }
+      if (iu < flo || iu + 31 > fhi) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = iu + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (!(i >= ilo && i <= ihi)) st[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] *= st[r];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const s16x8 pf = pack8<T>(st, h), sf = pack8<T>(dp, h);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          dv[dt] = mfma32<T>(col_frag32<D>(Dt, u * 32 + h * 16, dt), pf, dv[dt]);
+          dk[dt] = mfma32<T>(col_frag32<D>(Qt, u * 32 + h * 16, dt), sf, dk[dt]);
+        }
+      }
+    }
+  }
+  if (j >= s.nk) return;
+  char* pk = a.dk + (long long)(s.k0 + j) * a.lddk + pl.h * (D * 2);
+  char* pv = a.dv + (long long)(s.k0 + j) * a.lddv + pl.h * (D * 2);
+  typedef __attribute__((ext_vector_type(4))) T T4;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      T4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { x[e] = (T)(dk[dt][4 * g + e] * a.scale); y[e] = (T)dv[dt][4 * g + e]; }
+      *reinterpret_cast<T4*>(pk + (dt * 32 + 8 * g + 4 * half) * 2) = x;
+      *reinterpret_cast<T4*>(pv + (dt * 32 + 8 * g + 4 * half) * 2) = y;
+    }
+}
+
+static bool rows_wrong(const void* p, long long ld, int heads, int D) {
+  return !p || (uintptr_t)p % 16 || ld % 8 || ld < (long long)heads * D || ld > (1 << 22);
+}
+static int window_wrong(const char* what, const void* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D,
+                        int dtype, int sinks, float scale) {
+  const char* w = nullptr;
+  if (D != 64 && D != 128) w = "heads of 64 or 128 values";
+  else if (dtype != 0 && dtype != 1) w = "element type: 0 (bf16) or 1 (fp16)";
+  else if (Hkv < 1 || Hq < 1 || Hq % Hkv) w = "the query heads are not a multiple of the key heads";
+  else if (B < 0 || max_q < 0 || max_k < 0 || rows_q < 0 || rows_k < 0 || max_q > (1 << 29) || max_k > (1 << 29)) w = "lengths of 0 to 2^29";
+  else if (B && !seqs) w = "the table of sequences is missing";
+  else if ((uintptr_t)seqs % 16) w = "the table of sequences is not aligned to 16 bytes";
+  else if (sinks < 0 || sinks > (1 << 29)) w = "sinks of 0 to 2^29";
+  else if (!(scale > 0.f && scale < 1e30f)) w = "the scale is not a positive number";
+  else if ((long long)B * Hq * (max_q / 128 + 1) >= (1ll << 30) || (long long)B * Hkv * (max_k / 128 + 1) >= (1ll << 30)) w = "more than 2^30 tiles";
+  if (!w) return 0;
+  char msg[160];
+  snprintf(msg, sizeof msg, "%s: %s", what, w);
+  set_error(msg);
+  return -2;
+}
+static int far(int n) { return n < 0 || n > (1 << 29) ? 1 << 29 : n; }      // a window without that edge
+
+}  // namespace oat
+
+using namespace oat;
+
+#define WIN_LAUNCH(kernel, blocks)                                                                                   \
+  do {                                                                                                               \
+    const dim3 g_(place_grid(blocks));                                                                               \
+    if (dtype == 0 && D == 64) OAT_LAUNCH(kernel<bf16, 64>, g_, dim3(256), 0, s, a);                                 \
+    else if (dtype == 0) OAT_LAUNCH(kernel<bf16, 128>, g_, dim3(256), 0, s, a);                                      \
+    else if (D == 64) OAT_LAUNCH(kernel<_Float16, 64>, g_, dim3(256), 0, s, a);                                      \
+    else OAT_LAUNCH(kernel<_Float16, 128>, g_, dim3(256), 0, s, a);                                                  \
+  } while (0)
+
+extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
+                                   long long ldo, float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k,
+                                   int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* stream) {
+  if (int rc = window_wrong("attn_window_fwd", seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, sinks, scale)) return rc;
+  if (B == 0 || max_q == 0 || rows_q == 0) return 0;
+  if (rows_wrong(q, ldq, Hq, D) || rows_wrong(out, ldo, Hq, D) || (rows_k && (rows_wrong(k, ldk, Hkv, D) || rows_wrong(v, ldv, Hkv, D)))) {
+    set_error("attn_window_fwd: q, k, v, out need 16-byte aligned rows (pitch a multiple of 8, at least the heads, at most 2^22 values)");
+    return -2;
+  }
+  WinArgs a{};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)out; a.lse = lse;
+  a.ldq = ldq * 2; a.ldk = ldk * 2; a.ldv = ldv * 2; a.ldo = ldo * 2;
+  a.seqs = (const int4*)seqs;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
+  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
+  hipStream_t s = (hipStream_t)stream;
+  WIN_LAUNCH(win_fwd_kernel, (long long)B * Hq * ((max_q + 127) / 128));
+  return check_launch("attn_window_fwd");
+}
+
+extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int Hq) { return (size_t)rows_q * Hq * 8; }
+
+extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
+                                   long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
+                                   long long lddk, void* dv, long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q,
+                                   int rows_k, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = window_wrong("attn_window_bwd", seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, sinks, scale)) return rc;
+  if (B == 0) return 0;
+  if (rows_q && (rows_wrong(q, ldq, Hq, D) || rows_wrong(out, ldo, Hq, D) || rows_wrong(dout, lddo, Hq, D) || rows_wrong(dq, lddq, Hq, D) || !lse)) {
+    set_error("attn_window_bwd: q, out, dout, dq need 16-byte aligned rows (pitch a multiple of 8, at least the heads, at most 2^22 values), and lse");
+    return -2;
+  }
+  if (rows_k && (rows_wrong(k, ldk, Hkv, D) || rows_wrong(v, ldv, Hkv, D) || rows_wrong(dk, lddk, Hkv, D) || rows_wrong(dv, lddv, Hkv, D))) {
+    set_error("attn_window_bwd: k, v, dk, dv need 16-byte aligned rows (pitch a multiple of 8, at least the heads, at most 2^22 values)");
+    return -2;
+  }
+  if (rows_q && (!workspace || workspace_bytes < oat_attn_window_bwd_workspace_bytes(rows_q, Hq))) { set_error("attn_window_bwd: the workspace is too small"); return -3; }
+  WinArgs a{};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.dout = (const char*)dout;
+  a.lse = const_cast<float*>(lse); a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;
+  a.ldq = ldq * 2; a.ldk = ldk * 2; a.ldv = ldv * 2; a.ldo = ldo * 2; a.lddo = lddo * 2; a.lddq = lddq * 2; a.lddk = lddk * 2; a.lddv = lddv * 2;
+  a.lse2 = (float*)workspace; a.delta = a.lse2 + (size_t)rows_q * Hq;
+  a.seqs = (const int4*)seqs;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
+  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
+  hipStream_t s = (hipStream_t)stream;
+  if (max_q && rows_q) WIN_LAUNCH(win_bwd_q_kernel, (long long)B * Hq * ((max_q + 127) / 128));
+  if (max_k && rows_k) WIN_LAUNCH(win_bwd_kv_kernel, (long long)B * Hkv * ((max_k + 127) / 128));
+  return check_launch("attn_window_bwd");
+}

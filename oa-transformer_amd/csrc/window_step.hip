@@ -1,0 +1,351 @@
+// The serving form of windowed attention: one new token of every sequence against a cache of keys and values, and the copy of a
+// prompt's keys and values into such a cache.
+//
+// A cache holds `cap` slots per sequence.  Plain: token t stands in slot t.  Rolling: the first `sinks` tokens stay, the others go
+// round in the remaining slots, slot(t) = sinks + (t - sinks) mod (cap - sinks), so a window of cap - sinks tokens and the sinks is
+// all that is ever held.  The order of a softmax's terms is free, so the step never unrolls a rolling cache.
+#include "attn_window.h"
+
+namespace oat {
+
+template <class T> OAT_DEV f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c);
+template <> OAT_DEV f32x4 mfma16<bf16>(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> OAT_DEV f32x4 mfma16<_Float16>(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+struct StepArgs {
+  const char* qkv; long long ldqkv;                  // bytes; q heads | k heads | v heads
+  const int* past;                                   // [B] tokens before this one
+  const int* pos;                                    // [B, n_axes]
+  char *kc, *vc;
+  long long kb, ks, kh, vb, vs, vh;                  // cache strides in bytes: sequence, slot, head
+  char* out; long long ldo;
+  float* pieces; int* tickets;
+  int B, Hq, Hkv, cap, left, sinks, rolling, splits, turn;
+  float scale;
+  OatRope rope;
+};
+
+constexpr int SK = 32;                               // keys of a wave's tile
+template <int D> constexpr int step_lds() { return 4 * 2 * 2 * SK * D * 2; }
+
+// One workgroup = one piece of the visible keys of one (sequence, key head), for up to 16 of the query heads that share it; a wave
+// takes every fourth tile of 32 keys.  Bound: the cache is read once - HBM; so keys and values go straight to the LDS (asynchronous,
+// two tiles of each ahead per wave, no register waits on them) and each wave waits for its own tiles only.  S^T = K Q^T and
+// O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
+// The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the last piece writes the new
+// row to the cache first.  Pieces are joined by the workgroup that finishes last, in the order of the pieces.
+template <class T, int D>
+__global__ __launch_bounds__(256) void win_step_kernel(StepArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  __shared__ __attribute__((aligned(16))) T qs[16 * D];
+  __shared__ float2 cs[64];
+  __shared__ float wm[4][16], wl[4][16];
+  __shared__ int last;
+  constexpr int CPR = D / 8, NI = SK * CPR / 64, TB = SK * D * 2;
+  const int G = a.Hq / a.Hkv, gts = (G + 15) / 16;
+  const int piece = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+  const int gt = rest % gts, hk = rest / gts % a.Hkv, b = rest / gts / a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g0 = gt * 16, ng = min(16, G - g0);
+  const int p = a.past[b];
+  if (p < 0 || (!a.rolling && p >= a.cap)) {         // a sequence that takes no part (or has no slot left): zeros, the cache stays
+    if (piece == 0)
+      for (int t = tid; t < ng * D; t += 256) reinterpret_cast<T*>(a.out + b * a.ldo)[(hk * G + g0) * D + t] = (T)0.f;
+    return;
+  }
+  const int all = p < 0x7fffffff ? p + 1 : p;
+  const int nv = a.rolling ? min(all, a.cap) : (a.left < all - 1 - a.sinks ? a.sinks + a.left + 1 : all);
+  const int shift = a.rolling ? 0 : all - nv;
+  const int chunk = ((nv + a.splits - 1) / a.splits + 4 * SK - 1) / (4 * SK) * (4 * SK);
+  const int parts = (nv + chunk - 1) / chunk, ta = piece * chunk, tb = min(nv, ta + chunk);
+  if (ta >= nv) return;
+  const char* row = a.qkv + b * a.ldqkv;
+  const int np = a.turn ? a.rope.n_pairs : 0;
+  auto turned = [&](const T* x, int d) {             // value d of a head, turned
+    if (d >= 2 * np) return (float)x[d];
+    const int pr = a.rope.interleaved ? d >> 1 : d < np ? d : d - np;
+    const bool second = a.rope.interleaved ? d & 1 : d >= np;
+    const int iu = a.rope.interleaved ? 2 * pr : pr, iv = a.rope.interleaved ? 2 * pr + 1 : pr + np;
+    const float u = (float)x[iu], v = (float)x[iv];
+    return second ? v * cs[pr].x + u * cs[pr].y : u * cs[pr].x - v * cs[pr].y;
+  };
+  if (tid < np) cs[tid] = rope_cos_sin(a.pos[(size_t)b * a.rope.n_axes + a.rope.axis[tid]], a.rope.turns[tid], false);
+  __syncthreads();
+  char* kb = a.kc + b * a.kb + hk * a.kh;
+  char* vb = a.vc + b * a.vb + hk * a.vh;
+  if (tb == nv) {
+    const int slot = !a.rolling || p < a.sinks ? p : a.sinks + (p - a.sinks) % (a.cap - a.sinks);
+    if (tid < D) {
+      reinterpret_cast<T*>(kb + slot * a.ks)[tid] = (T)turned(reinterpret_cast<const T*>(row) + (a.Hq + hk) * D, tid);
+      reinterpret_cast<T*>(vb + slot * a.vs)[tid] = reinterpret_cast<const T*>(row)[(a.Hq + a.Hkv + hk) * D + tid];
+    }
+  }
+  for (int t = tid; t < 16 * D; t += 256) {
+    const int g = t / D, d = t % D;
+    qs[t] = g < ng ? (T)turned(reinterpret_cast<const T*>(row) + (hk * G + g0 + g) * D, d) : (T)0.f;
+  }
+  tile_barrier();                                    // the new row has been written before any wave reads it
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds) + wave * 4 * TB;
+  char* const mine = lds + wave * 4 * TB;
+  auto stage = [&](int t0, int buf) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = i * 64 + lane, r = c / CPR, ch = (c % CPR) ^ swz<D>(r);
+      const int t = min(t0 + r, tb - 1);
+      const long long slot = t < a.sinks ? t : t + shift;
+      const uint32_t dst = l0 + buf * 2 * TB + i * 1024;
+      uint32_t keep;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                   "s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                   : "=&s"(keep) : "v"(kb + slot * a.ks + ch * 16), "v"(vb + slot * a.vs + ch * 16), "s"(dst), "s"(dst + TB) : "memory");
+    }
+  };
+  const int gq = lane >> 4, r16 = lane & 15;
+  const float c = a.scale * LOG2E;
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  int t0 = ta + wave * SK, buf = 0;
+  if (t0 < tb) stage(t0, 0);
+  for (; t0 < tb; t0 += 4 * SK, buf ^= 1) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t0 + 4 * SK < tb) {
+      stage(t0 + 4 * SK, buf ^ 1);
+      if constexpr (NI == 8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const char* Kt = mine + buf * 2 * TB;
+    const char* Vt = Kt + TB;
+    f32x4 st[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      st[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) {
+        const s16x8 kf = *reinterpret_cast<const s16x8*>(Kt + (u * 16 + r16) * (D * 2) + (((4 * ks + gq) ^ swz<D>(r16)) << 4));
+        const s16x8 qf = *reinterpret_cast<const s16x8*>(qs + r16 * D + ks * 32 + gq * 8);
+        st[u] = mfma16<T>(kf, qf, st[u]);
+      }
+    }
+    if (t0 + SK > tb) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t0 + u * 16 + 4 * gq + r >= tb) st[u][r] = -INFINITY;
+    }
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[u][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float al = __builtin_amdgcn_exp2f((m - mx) * c);            // mx is finite: a tile holds one visible key at least
+    m = mx;
+    l *= al;
+    typedef __attribute__((ext_vector_type(8))) T T8;
+    T8 pf;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f((st[u][r] - mx) * c);
+        l += e;
+        pf[4 * u + r] = (T)e;
+      }
+    const int j = (lane >> 2) & 3, q4 = lane & 3;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      s16x8 vf;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 4 * gq + j;
+        const s16x4 h = lds_tr16(Vt + (16 * e + r) * (D * 2) + (((2 * dt + (q4 >> 1)) ^ swz<D>(r)) << 4) + (q4 & 1) * 8);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vf[4 * e + x] = h[x];
+      }
+      o[dt] *= al;
+      o[dt] = mfma16<T>(vf, __builtin_bit_cast(s16x8, pf), o[dt]);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  // the four waves' sums meet in the LDS: [wave][head][D]
+  __syncthreads();
+  float* os = reinterpret_cast<float*>(lds);
+  if (gq == 0) { wm[wave][r16] = m; wl[wave][r16] = l; }
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(os + (wave * 16 + r16) * D + dt * 16 + 4 * gq) = o[dt];
+  __syncthreads();
+  for (int t = tid; t < ng * D; t += 256) {
+    const int g = t / D, d = t % D;
+    float mm = wm[0][g];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mm = fmaxf(mm, wm[w][g]);
+    float ll = 0.f, oo = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = __builtin_amdgcn_exp2f((wm[w][g] - mm) * c);
+      ll += wl[w][g] * e;
+      oo += os[(w * 16 + g) * D + d] * e;
+    }
+    const int h = hk * G + g0 + g;
+    if (parts == 1) {
+      reinterpret_cast<T*>(a.out + b * a.ldo)[h * D + d] = (T)(oo / ll);
+    } else {
+      float* pc = a.pieces + ((size_t)(b * a.Hq + h) * a.splits + piece) * (D + 2);
+      pc[d] = oo;
+      if (d == 0) { pc[D] = mm * c; pc[D + 1] = ll; }
+    }
+  }
+  if (parts == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    int* tk = a.tickets + b * a.Hkv + hk;
+    last = atomicAdd(tk, 1) == parts * gts - 1;
+    if (last) atomicExch(tk, 0);
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int t = tid; t < G * D; t += 256) {
+    const int h = hk * G + t / D, d = t % D;
+    const float* pc = a.pieces + (size_t)(b * a.Hq + h) * a.splits * (D + 2);
+    float mm = -INFINITY;
+    for (int i = 0; i < parts; ++i) mm = fmaxf(mm, pc[i * (D + 2) + D]);
+    float ll = 0.f, oo = 0.f;
+    for (int i = 0; i < parts; ++i) {
+      const float e = __builtin_amdgcn_exp2f(pc[i * (D + 2) + D] - mm);
+      ll += pc[i * (D + 2) + D + 1] * e;
+      oo += pc[i * (D + 2) + d] * e;
+    }
+    reinterpret_cast<T*>(a.out + b * a.ldo)[h * D + d] = (T)(oo / ll);
+  }
+}
+
+// ---- a prompt's keys and values into a cache: slot by slot, the token that holds it at the end (no two writers of a slot)
+struct FillArgs {
+  const char *k, *v;
+  long long ldk, ldv;
+  char *kc, *vc;
+  long long kb, ks, kh, vb, vs, vh;
+  const int4* seqs;
+  int B, Hkv, cap, sinks, rows_k, chunks;            // chunks: 16-byte pieces of a head
+};
+__global__ __launch_bounds__(256) void cache_fill_kernel(FillArgs a) {
+  const int b = blockIdx.y, per = a.Hkv * a.chunks;
+  const int4 s = a.seqs[b];
+  if (s.z < 0 || s.w < 0 || (long long)s.z + s.w > a.rows_k) return;
+  const int S = min(a.sinks, a.cap), W = a.cap - S;
+  const long long total = (long long)min(a.cap, s.w) * per;
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+    const int slot = (int)(t / per), c = (int)(t - (long long)slot * per), h = c / a.chunks, x = c - h * a.chunks;
+    const int tok = slot < S ? slot : slot + (s.w - 1 - slot) / W * W;
+    const long long row = s.z + tok;
+    *reinterpret_cast<f32x4*>(a.kc + b * a.kb + slot * a.ks + h * a.kh + x * 16) = *reinterpret_cast<const f32x4*>(a.k + row * a.ldk + c * 16);
+    *reinterpret_cast<f32x4*>(a.vc + b * a.vb + slot * a.vs + h * a.vh + x * 16) = *reinterpret_cast<const f32x4*>(a.v + row * a.ldv + c * 16);
+  }
+}
+
+static int fail(const char* what, const char* why) {
+  char msg[192];
+  snprintf(msg, sizeof msg, "%s: %s", what, why);
+  set_error(msg);
+  return -2;
+}
+static const char* cache_wrong(const void* k, const void* v, const long long* st, int B, int cap, int Hkv, int D, int sinks) {
+  if (D != 64 && D != 128) return "heads of 64 or 128 values";
+  if (B < 0 || Hkv < 1 || cap < 1 || cap > (1 << 29) || sinks < 0 || sinks > (1 << 29)) return "no key heads, or a cache of no slots (or more than 2^29)";
+  if (!k || !v || !st) return "the cache is missing";
+  if (((uintptr_t)k | (uintptr_t)v) % 16) return "the cache is not aligned to 16 bytes";
+  for (int i = 0; i < 6; ++i)
+    if (st[i] < 0 || st[i] % 8) return "the cache's strides are not multiples of 8 values";
+  return nullptr;
+}
+// pieces a cache may be split into: about four workgroups per CU in all
+static int most_pieces(int B, int Hkv) { return min(256, 1 + 1024 / max(1, B * Hkv)); }
+
+}  // namespace oat
+
+using namespace oat;
+
+extern "C" size_t oat_attn_window_step_workspace_bytes(int B, int Hq, int Hkv, int D) {
+  if (B < 1 || Hq < 1 || Hkv < 1) return 0;
+  return ((size_t)B * Hq * most_pieces(B, Hkv) * (D + 2) + (size_t)B * Hkv) * 4;
+}
+
+extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int* past, void* kc, void* vc, const long long* strides, int cap,
+                                    void* out, long long ldo, int B, int Hq, int Hkv, int D, int dtype, int left, int sinks, int rolling,
+                                    float scale, const OatRope* rope, const int* pos, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* me = "attn_window_step";
+  if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
+  if (dtype != 0 && dtype != 1) return fail(me, "element type: 0 (bf16) or 1 (fp16)");
+  if (Hq < 1 || Hq % Hkv) return fail(me, "the query heads are not a multiple of the key heads");
+  if (!(scale > 0.f && scale < 1e30f)) return fail(me, "the scale is not a positive number");
+  if (B == 0) return 0;
+  if (!qkv || !out || !past) return fail(me, "qkv, out and the counts of past tokens are needed");
+  if (((uintptr_t)qkv | (uintptr_t)out) % 16 || ldqkv % 8 || ldo % 8 || ldqkv < (long long)(Hq + 2 * Hkv) * D || ldo < (long long)Hq * D)
+    return fail(me, "qkv and out need 16-byte aligned rows of all their heads");
+  if (rolling && (sinks >= cap || (left >= 0 && left != cap - sinks - 1))) return fail(me, "a rolling cache has sinks + left + 1 slots");
+  if (rope) {
+    if (const char* w = rope_wrong(rope, D)) return fail(me, w);
+    if (!pos) return fail(me, "positions are needed to turn by");
+  }
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < oat_attn_window_step_workspace_bytes(B, Hq, Hkv, D))
+    return fail(me, "the workspace is too small, or not aligned to 16 bytes");
+  if ((long long)B * Hkv * ((Hq / Hkv + 15) / 16) * most_pieces(B, Hkv) >= (1ll << 31)) return fail(me, "more than 2^31 pieces");
+  StepArgs a{};
+  a.qkv = (const char*)qkv; a.ldqkv = ldqkv * 2; a.past = past; a.pos = pos;
+  a.kc = (char*)kc; a.vc = (char*)vc;
+  a.kb = strides[0] * 2; a.ks = strides[1] * 2; a.kh = strides[2] * 2; a.vb = strides[3] * 2; a.vs = strides[4] * 2; a.vh = strides[5] * 2;
+  a.out = (char*)out; a.ldo = ldo * 2;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.cap = cap; a.sinks = sinks; a.rolling = rolling != 0;
+  a.left = left < 0 || left > (1 << 29) ? 1 << 29 : left;
+  const long long seen = rolling ? cap : min((long long)cap, (long long)sinks + a.left + 1);
+  a.splits = (int)max(1ll, min((long long)most_pieces(B, Hkv), (seen + 255) / 256));
+  a.turn = rope != nullptr;
+  if (rope) a.rope = *rope;
+  a.scale = scale;
+  a.tickets = (int*)workspace;
+  a.pieces = (float*)workspace + (size_t)B * Hkv;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)(B * Hkv * ((Hq / Hkv + 15) / 16) * a.splits));
+#define STEP_LAUNCH(T, DD)                                                       \
+  do {                                                                           \
+    OAT_MAX_LDS((win_step_kernel<T, DD>), step_lds<DD>());                        \
+    OAT_LAUNCH(win_step_kernel<T, DD>, grid, dim3(256), step_lds<DD>(), s, a);    \
+  } while (0)
+  if (dtype == 0 && D == 64) STEP_LAUNCH(bf16, 64);
+  else if (dtype == 0) STEP_LAUNCH(bf16, 128);
+  else if (D == 64) STEP_LAUNCH(_Float16, 64);
+  else STEP_LAUNCH(_Float16, 128);
+#undef STEP_LAUNCH
+  return check_launch(me);
+}
+
+extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k,
+                                     int max_k, void* kc, void* vc, const long long* strides, int cap, int Hkv, int D, int sinks,
+                                     void* stream) {
+  const char* me = "window_cache_fill";
+  if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
+  if (rows_k < 0 || max_k < 0 || B > 65535) return fail(me, "no rows, or more than 65535 sequences");
+  if (B == 0 || rows_k == 0 || max_k == 0) return 0;
+  if (!k || !v || !seqs || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)seqs) % 16 || ldk % 8 || ldv % 8 || ldk < (long long)Hkv * D || ldv < (long long)Hkv * D)
+    return fail(me, "k, v need 16-byte aligned rows of all key heads, and the table of sequences 16 bytes");
+  FillArgs a{};
+  a.k = (const char*)k; a.v = (const char*)v; a.ldk = ldk * 2; a.ldv = ldv * 2; a.kc = (char*)kc; a.vc = (char*)vc;
+  a.kb = strides[0] * 2; a.ks = strides[1] * 2; a.kh = strides[2] * 2; a.vb = strides[3] * 2; a.vs = strides[4] * 2; a.vh = strides[5] * 2;
+  a.seqs = (const int4*)seqs;
+  a.B = B; a.Hkv = Hkv; a.cap = cap; a.sinks = sinks; a.rows_k = rows_k; a.chunks = D / 8;
+  const long long n = (long long)min(cap, max_k) * Hkv * a.chunks;
+  OAT_LAUNCH(cache_fill_kernel, dim3((unsigned)min((n + 255) / 256, 4096ll), B), dim3(256), 0, (hipStream_t)stream, a);
+  return check_launch(me);
+}
