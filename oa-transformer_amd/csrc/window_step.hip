@@ -36,8 +36,8 @@ template <int D> constexpr int step_lds() { return 4 * 2 * 2 * SK * D * 2; }
 // takes every fourth tile of 32 keys.  Bound: the cache is read once - HBM; so keys and values go straight to the LDS (asynchronous,
 // two tiles of each ahead per wave, no register waits on them) and each wave waits for its own tiles only.  S^T = K Q^T and
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
-// The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the last piece writes the new
-// row to the cache first.  Pieces are joined by the workgroup that finishes last, in the order of the pieces.
+// The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
+// new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in the order of the pieces.
 template <class T, int D>
 __global__ __launch_bounds__(256) void win_step_kernel(StepArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -76,8 +76,9 @@ __global__ __launch_bounds__(256) void win_step_kernel(StepArgs a) {
   __syncthreads();
   char* kb = a.kc + b * a.kb + hk * a.kh;
   char* vb = a.vc + b * a.vb + hk * a.vh;
-  if (tb == nv) {
-    const int slot = !a.rolling || p < a.sinks ? p : a.sinks + (p - a.sinks) % (a.cap - a.sinks);
+  const int slot = !a.rolling || p < a.sinks ? p : a.sinks + (p - a.sinks) % (a.cap - a.sinks);
+  const int mark = a.rolling ? slot : nv - 1;        // where the new token stands among the visible ones
+  if (mark >= ta && mark < tb) {
     if (tid < D) {
       reinterpret_cast<T*>(kb + slot * a.ks)[tid] = (T)turned(reinterpret_cast<const T*>(row) + (a.Hq + hk) * D, tid);
       reinterpret_cast<T*>(vb + slot * a.vs)[tid] = reinterpret_cast<const T*>(row)[(a.Hq + a.Hkv + hk) * D + tid];

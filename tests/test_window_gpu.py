@@ -1,9 +1,10 @@
 """Rotary positions, windowed attention (forward, backward) and its one-token form on a real MI355X against their definitions in 64
-bits (oracle/window_oracle.py) on the same 16-bit inputs.
+bits (oracle/window_oracle.py, on the same device) on the same 16-bit inputs.
 
 Tolerances, with u = finfo(dtype).eps / 2 (half a step): an output is rounded once (u |value|), and a product of two 16-bit operands
 of which one is a rounded probability (or its gradient) is off by u times the sum of its terms' absolute values (the oracle's
-*_abs); 2^-14 of that sum stands for sums, exponentials and the log-sum-exp in 32 bits."""
+*_abs) at most.  The terms' roundings are independent, each at most u: their sum stays within 6 u times the root of the sum of the terms'
+squares (*_sq; six deviations or more), and the smaller of the two bounds is taken.  2^-14 of *_abs stands for sums, exponentials and the log-sum-exp in 32 bits."""
 import math
 
 import pytest
@@ -32,8 +33,13 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def terms(r, name, u):
+    """how far a sum with 16-bit terms may be off (see above)"""
+    return torch.minimum(u * r[name + "_abs"], 6 * u * r[name + "_sq"]) + 2.0 ** -14 * r[name + "_abs"]
+
+
 def within(got, ref, tol, what):
-    got = got.double().cpu()
+    got, tol = got.double(), tol.expand_as(ref) if isinstance(tol, torch.Tensor) else tol
     bad = ~((got - ref).abs() <= tol)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} beyond the bound; worst {float(((got - ref).abs() - tol)[bad].max()):.3g} over, "
                            f"at {bad.nonzero()[0].tolist()}: {got[tuple(bad.nonzero()[0])]} for {ref[tuple(bad.nonzero()[0])]}")
@@ -58,14 +64,14 @@ def test_rope_axes(case, dtype):
         pos = torch.randint(-5000, 2_000_000, (P, len(sections)), generator=g, dtype=torch.int32)
         for inverse in (False, True):
             out = hip.rope_axes(x, pos.to(DEV), rope, heads, dim, inverse=inverse)
-            ref = wo.rope(x.cpu().view(M, heads, dim) if x.is_contiguous() else x.cpu().reshape(M, heads, dim), pos.repeat(M // P, 1), sections,
+            ref = wo.rope(x.reshape(M, heads, dim), pos.repeat(M // P, 1).to(DEV), sections,
                           theta, shared, inter, inverse).reshape(M, -1)
             # cos and sin in 32 bits (a few 2^-24 of the pair's length), one rounding of the result
-            size = x.double().cpu().reshape(M, heads, dim).abs().amax(-1, keepdim=True).expand(M, heads, dim).reshape(M, -1)
+            size = x.double().reshape(M, heads, dim).abs().amax(-1, keepdim=True).expand(M, heads, dim).reshape(M, -1)
             within(out, ref, half_step(dtype) * ref.abs() + 2.0 ** -21 * size + torch.finfo(dtype).tiny, f"rope {M}")
         back = hip.rope_axes(out, pos.to(DEV), rope, heads, dim, out=out)          # in place, the turn back of the inverse
         assert back is out
-        within(out, x.double().cpu(), 3 * half_step(dtype) * size * 1.5 + 2.0 ** -20 * size, "rope back")
+        within(out, x.double(), 3 * half_step(dtype) * size * 1.5 + 2.0 ** -20 * size, "rope back")
         assert torch.equal(wide[:, heads * dim:], rnd(M, heads * dim + 8, dtype=dtype, seed=case)[:, heads * dim:])
 
 
@@ -77,12 +83,12 @@ def test_rope_axes_unaligned_rows_and_gradient():
     x = flat[1:].view(33, 193)[:, :192]                                             # 4-byte aligned rows of an odd pitch
     pos = torch.randint(0, 400, (33, 3), dtype=torch.int32)
     out = hip.rope_axes(x, pos.to(DEV), rope, 3, 64)
-    ref = wo.rope(x.cpu().reshape(33, 3, 64), pos, (16, 24, 24), 10000.0).reshape(33, -1)
+    ref = wo.rope(x.reshape(33, 3, 64), pos.to(DEV), (16, 24, 24), 10000.0).reshape(33, -1)
     within(out, ref, 2.0 ** -20 * x.double().abs().max().item() * torch.ones_like(ref), "unaligned")
     leaf = x.detach().clone().contiguous().requires_grad_(True)
     w = rnd(33, 192, dtype=torch.float32, seed=5)
     (g,) = torch.autograd.grad((wa.rope_axes(leaf, pos.to(DEV), rope, 3, 64) * w).sum(), leaf)
-    ref = wo.rope(w.cpu().reshape(33, 3, 64), pos, (16, 24, 24), 10000.0, inverse=True).reshape(33, -1)
+    ref = wo.rope(w.reshape(33, 3, 64), pos.to(DEV), (16, 24, 24), 10000.0, inverse=True).reshape(33, -1)
     within(g, ref, 2.0 ** -20 * w.double().abs().max().item() * torch.ones_like(ref), "gradient")
 
 
@@ -141,23 +147,23 @@ def test_attn_window(n, dtype):
     dq, dk, dv = (torch.full((t.shape[0], t.shape[1] + 8), 7.0, dtype=dtype, device=DEV)[:, :t.shape[1]] for t in (q, k, v))
     hip.attn_window_bwd(q, k, v, out, lse, do, table, Hq, Hkv, D, mq, mk, left, right, sinks, scale, dq=dq, dk=dk, dv=dv)
     r = wo.attention(q, k, v, seqs, Hq, Hkv, D, left, right, sinks, scale, dout=do, out=out)
-    u, e = half_step(dtype), 2.0 ** -14
+    u = half_step(dtype)
     tiny = torch.finfo(dtype).tiny                                                     # what rounds to a subnormal or to zero
     sq, sk = r["seen_q"], r["seen_k"]
-    within(out[sq.to(DEV)], r["out"][sq], (u * r["out"].abs() + (u + e) * r["out_abs"])[sq] + tiny, "out")
+    within(out[sq], r["out"][sq], (u * r["out"].abs() + terms(r, "out", u))[sq] + tiny, "out")
     some = r["lse"] > -math.inf
-    within(lse.cpu()[sq[:, None] & some], r["lse"][sq[:, None] & some], 2.0 ** -17 * (4 + r["lse"].abs())[sq[:, None] & some], "lse")
-    assert (lse.cpu()[sq[:, None] & ~some] == -math.inf).all()
-    within(dq[sq.to(DEV)], r["dq"][sq], (u * r["dq"].abs() + (u + e) * r["dq_abs"] + 1.01 * r["dq_off"])[sq] + tiny * D, "dq")
-    within(dk[sk.to(DEV)], r["dk"][sk], (u * r["dk"].abs() + (u + e) * r["dk_abs"] + 1.01 * r["dk_off"])[sk] + tiny * (8 + mq), "dk")
-    within(dv[sk.to(DEV)], r["dv"][sk], (u * r["dv"].abs() + (u + e) * r["dv_abs"])[sk] + tiny * (8 + mq), "dv")
+    within(lse[sq[:, None] & some], r["lse"][sq[:, None] & some], 2.0 ** -17 * (4 + r["lse"].abs())[sq[:, None] & some], "lse")
+    assert (lse[sq[:, None] & ~some] == -math.inf).all()
+    within(dq[sq], r["dq"][sq], (u * r["dq"].abs() + terms(r, "dq", u) + 1.01 * r["dq_off"])[sq] + tiny * D, "dq")
+    within(dk[sk], r["dk"][sk], (u * r["dk"].abs() + terms(r, "dk", u) + 1.01 * r["dk_off"])[sk] + tiny * (8 + mq), "dk")
+    within(dv[sk], r["dv"][sk], (u * r["dv"].abs() + terms(r, "dv", u))[sk] + tiny * (8 + mq), "dv")
     for t, s in ((out, sq), (lse, sq), (dq, sq), (dk, sk), (dv, sk)):                  # rows of no sequence stay as they were
-        assert (t[~s.to(DEV)] == 7.0).all()
+        assert (t[~s] == 7.0).all()
     # every sum has one order
     again = [torch.zeros_like(t) for t in (dq, dk, dv)]
     hip.attn_window_bwd(q, k, v, out, lse, do, table, Hq, Hkv, D, mq, mk, left, right, sinks, scale, dq=again[0], dk=again[1], dv=again[2])
     for a, b, s in zip(again, (dq, dk, dv), (sq, sk, sk)):
-        assert torch.equal(a[s.to(DEV)], b[s.to(DEV)])
+        assert torch.equal(a[s], b[s])
 
 
 def test_attn_window_large_and_equal_scores():
@@ -167,8 +173,8 @@ def test_attn_window_large_and_equal_scores():
     v = rnd(200, 64, seed=1)
     q = torch.zeros(200, 64, dtype=BF, device=DEV)
     out = hip.attn_window_fwd(q, q, v, table, 1, 1, 64, 200, 200, right=-1)
-    mean = v.double().cpu().mean(0).expand(200, 64)
-    within(out, mean, half_step(BF) * mean.abs() + (half_step(BF) + 2.0 ** -14) * v.double().cpu().abs().mean(0), "mean")
+    mean = v.double().mean(0).expand(200, 64)
+    within(out, mean, half_step(BF) * mean.abs() + (half_step(BF) + 2.0 ** -14) * v.double().abs().mean(0), "mean")
     eye = torch.zeros(200, 64, dtype=BF, device=DEV)
     eye[torch.arange(200), torch.arange(200) % 64] = 128.0
     out = hip.attn_window_fwd(eye[:64].contiguous(), eye[:64].contiguous(), v[:64].contiguous(), hip.seq_table([64]), 1, 1, 64, 64, 64, right=-1)
@@ -232,15 +238,15 @@ def test_window_attention_gradient_with_rope(padded):
     qk = hip.rope_axes(qkv.detach()[:, :n], pos.to(DEV), rope, Hq + Hkv, D)
     seqs = [tuple(t) for t in table.tolist()]
     r = wo.attention(qk[:, :Hq * D], qk[:, Hq * D:], qkv.detach()[:, n:], seqs, Hq, Hkv, D, left, right, sinks, D ** -0.5, dout=dout, out=out.detach())
-    u, e = half_step(BF), 2.0 ** -14
-    within(out.detach(), r["out"], u * r["out"].abs() + (u + e) * r["out_abs"] + 1e-30, "out")
-    back = wo.rope(torch.cat([r["dq"], r["dk"]], 1).view(M, Hq + Hkv, D), pos, sections, 10000.0, inverse=True).view(M, n)
-    tol = torch.cat([u * r["dq"].abs() + (u + e) * r["dq_abs"] + 1.01 * r["dq_off"], u * r["dk"].abs() + (u + e) * r["dk_abs"] + 1.01 * r["dk_off"]], 1)
+    u = half_step(BF)
+    within(out.detach(), r["out"], u * r["out"].abs() + terms(r, "out", u) + 1e-30, "out")
+    back = wo.rope(torch.cat([r["dq"], r["dk"]], 1).view(M, Hq + Hkv, D), pos.to(DEV), sections, 10000.0, inverse=True).view(M, n)
+    tol = torch.cat([u * r["dq"].abs() + terms(r, "dq", u) + 1.01 * r["dq_off"], u * r["dk"].abs() + terms(r, "dk", u) + 1.01 * r["dk_off"]], 1)
     # the turn mixes a pair's errors (at most their sum) and rounds once more
     pair = tol.view(M, Hq + Hkv, 2, 32)
     tol = (pair + pair.flip(2)).view(M, n) + u * back.abs() * 1.1
     within(g[:, :n], back, tol + 1e-30, "dq | dk")
-    within(g[:, n:], r["dv"], u * r["dv"].abs() + (u + e) * r["dv_abs"] + 1e-30, "dv")
+    within(g[:, n:], r["dv"], u * r["dv"].abs() + terms(r, "dv", u) + 1e-30, "dv")
     if padded:
         assert (out[90 + 33:] == 0).all() and (g[90 + 33:] == 0).all()
 
@@ -252,17 +258,17 @@ def test_window_attention_gradient_by_differences():
     M, D = 40, 64
     table = hip.seq_table([M])
     qkv = rnd(M, 3 * D, dtype=HF, seed=8).requires_grad_(True)
-    w, d = rnd(M, D, dtype=HF, seed=9), rnd(M, 3 * D, dtype=torch.float64, seed=10).cpu()
+    w, d = rnd(M, D, dtype=HF, seed=9), rnd(M, 3 * D, dtype=torch.float64, seed=10)
     out = wa.window_attention(qkv, table, 1, 1, D, left=11, right=0, sinks=2, longest=M)
     (g,) = torch.autograd.grad(out, qkv, w)
 
     def f(x):
-        return (wo.attention(x[:, :D], x[:, D:2 * D], x[:, 2 * D:], [(0, M, 0, M)], 1, 1, D, 11, 0, 2, D ** -0.5)["out"] * w.double().cpu()).sum()
-    x, h = qkv.detach().double().cpu(), 1e-5
+        return (wo.attention(x[:, :D], x[:, D:2 * D], x[:, 2 * D:], [(0, M, 0, M)], 1, 1, D, 11, 0, 2, D ** -0.5)["out"] * w.double()).sum()
+    x, h = qkv.detach().double(), 1e-5
     diff = float(f(x + h * d) - f(x - h * d)) / (2 * h)
     # the gradient's roundings: a few half steps (2^-11) of its size, in random directions
-    size = float((g.double().cpu() * d).norm())
-    assert abs(float((g.double().cpu() * d).sum()) - diff) <= 6 * 2.0 ** -11 * size * math.sqrt(3 * M * D) / 8, (diff, float((g.double().cpu() * d).sum()))
+    size = float((g.double() * d).norm())
+    assert abs(float((g.double() * d).sum()) - diff) <= 6 * 2.0 ** -11 * size * math.sqrt(3 * M * D) / 8, (diff, float((g.double() * d).sum()))
 
 
 # ---------------------------------------------------------------------------------------------- one token
@@ -284,22 +290,22 @@ STEP = [
 
 
 def _step_ref(qkv, kc, vc, past, Hq, Hkv, D, left, sinks, rolling, scale, rope, sections, pos):
-    """-> out, abs, caches with the new rows as this dtype holds them"""
+    """-> out, its abs and sq, caches with the new rows as this dtype holds them"""
     B, cap = kc.shape[:2]
-    x = qkv.cpu().view(B, Hq + 2 * Hkv, D)
+    x = qkv.reshape(B, Hq + 2 * Hkv, D)
     kc, vc = kc.clone(), vc.clone()
-    out, size = torch.zeros(B, Hq, D, dtype=torch.float64), torch.zeros(B, Hq, D, dtype=torch.float64)
+    out, size, sq = (torch.zeros(B, Hq, D, dtype=torch.float64, device=DEV) for _ in range(3))
     for b, p in enumerate(past):
         if p < 0 or (not rolling and p >= cap):
             continue
         qk = x[b:b + 1, :Hq + Hkv].double()
         if rope is not None:
-            qk = wo.rope(qk, pos[b:b + 1], sections, rope.theta, rope.shared, rope.interleaved)
+            qk = wo.rope(qk, pos[b:b + 1].to(DEV), sections, rope.theta, rope.shared, rope.interleaved)
         qk = qk[0].to(kc.dtype)
         s = wo.slot(p, cap, sinks, rolling)
         kc[b, s], vc[b, s] = qk[Hq:], x[b, Hq + Hkv:]
-        out[b], size[b] = wo.step(qk[:Hq], kc[b], vc[b], p, left, sinks, rolling, scale)
-    return out.view(B, -1), size.view(B, -1), kc, vc
+        out[b], size[b], sq[b] = wo.step(qk[:Hq], kc[b], vc[b], p, left, sinks, rolling, scale)
+    return out.view(B, -1), {"out_abs": size.view(B, -1), "out_sq": sq.view(B, -1)}, kc, vc
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -307,7 +313,7 @@ def _step_ref(qkv, kc, vc, past, Hq, Hkv, D, left, sinks, rolling, scale, rope, 
 def test_attn_window_step(n, dtype):
     hip = _hip()
     B, cap, Hq, Hkv, D, left, sinks, rolling, past = STEP[n]
-    u, e = half_step(dtype), 2.0 ** -14
+    u = half_step(dtype)
     pieces = hip.window_step_workspace(B, Hq, Hkv, D)
     for turn in (None, ((D,), False), ((16, 24, 24), True)):
         qkv = rnd(B, (Hq + 2 * Hkv) * D + 16, dtype=dtype, seed=n)[:, :(Hq + 2 * Hkv) * D]
@@ -315,20 +321,38 @@ def test_attn_window_step(n, dtype):
         rope = hip.RopeAxes(turn[0], interleaved=turn[1]) if turn else None
         pos = torch.randint(0, 3000, (B, len(turn[0])), dtype=torch.int32) if turn else None
         scale = 1.1 / math.sqrt(D)
-        ref, size, kr, vr = _step_ref(qkv, kc.cpu(), vc.cpu(), past, Hq, Hkv, D, left, sinks, rolling, scale, rope, turn and turn[0], pos)
+        ref, r, kr, vr = _step_ref(qkv, kc, vc, past, Hq, Hkv, D, left, sinks, rolling, scale, rope, turn and turn[0], pos)
         # the turned query and key are the operator's own 16-bit values: one of them may fall on the other side of a border (32-bit angles),
         # which moves a score by a step of one term, 2 u |q k| scale <= 2^-5 u of the probabilities' size at these magnitudes
         for _ in range(2):                                                            # the workspace is ready again after a call
             out = hip.attn_window_step(qkv, torch.tensor(past, dtype=torch.int32, device=DEV), kc, vc, Hq, left=left, sinks=sinks, rolling=rolling,
                                        scale=scale, rope=rope, pos=pos.to(DEV) if turn else None, pieces=pieces)
-            within(out, ref, u * ref.abs() + (u * (1 + (2.0 if turn else 0.0)) + e) * size + torch.finfo(dtype).tiny, f"step {turn}")
-        assert torch.equal(vc.cpu(), vr)
+            within(out, ref, u * ref.abs() + terms(r, "out", u) + (2 * u * r["out_abs"] if turn else 0.0) + torch.finfo(dtype).tiny, f"step {turn}")
+        assert torch.equal(vc, vr)
         if turn:
             within(kc, kr.double(), 2 * u * kr.double().abs() + 2.0 ** -20, "cache")
         else:
-            assert torch.equal(kc.cpu(), kr)
+            assert torch.equal(kc, kr)
         same = [b for b, p in enumerate(past) if p < 0 or (not rolling and p >= cap)]
         assert all((out[b] == 0).all() for b in same)
+
+
+@pytest.mark.parametrize("cap,sinks,rolling", [(1500, 4, True), (1500, 0, True), (1500, 4, False), (4000, 700, True)])
+def test_attn_window_step_sees_its_own_token(cap, sinks, rolling):
+    """The new token's key points where the query does and takes nearly all of the weight: its value is the output, whichever piece of
+    the cache its slot falls into."""
+    hip = _hip()
+    D = 64
+    pieces = hip.window_step_workspace(1, 1, 1, D)
+    for past in (0, 3, 255, 256, 700, cap - 1, cap, cap + 255, cap + 900, 3 * cap):
+        if not rolling and past >= cap:
+            continue
+        kc, vc = rnd(1, cap, 1, D, seed=past), rnd(1, cap, 1, D, seed=past + 1)
+        qkv = rnd(1, 3 * D, seed=past + 2)
+        qkv[:, D:2 * D] = 8 * qkv[:, :D]                     # its score is 8 |q|^2 / 8 ~ 64, the others' ~ 1: e^-50 is left for them
+        out = hip.attn_window_step(qkv, torch.tensor([past], dtype=torch.int32, device=DEV), kc, vc, 1, sinks=sinks, rolling=rolling, pieces=pieces)
+        v = qkv[:, 2 * D:].double()
+        within(out, v, 2.0 ** -20 * v.abs() + 1e-6, f"past {past}")
 
 
 def test_attn_window_step_far_slots():
@@ -343,7 +367,7 @@ def test_attn_window_step_far_slots():
     ks, vs = torch.cat([kc[:, :4], kc[:, -300:]], 1).contiguous(), torch.cat([vc[:, :4], vc[:, -300:]], 1).contiguous()
     ref = hip.attn_window_step(qkv, torch.tensor([303], dtype=torch.int32, device=DEV), ks, vs, 8, left=299, sinks=4)
     u = half_step(BF)
-    within(out, ref.double().cpu(), 4 * u * ref.double().cpu().abs() + 4 * u * vs.double().abs().max().item(), "far")
+    within(out, ref.double(), 4 * u * ref.double().abs() + 4 * u * vs.double().abs().max().item(), "far")
 
 
 @pytest.mark.parametrize("cap,sinks,lens", [(40, 0, [40, 1]), (20, 4, [19, 20, 21, 100]), (16, 15, [3, 200]), (5, 9, [4, 5])])
@@ -386,11 +410,11 @@ def test_prompt_then_steps_is_one_long_attention(window, slots, sinks, axes):
         for b in range(2):
             got[b].append(o[b:b + 1])
     assert cache.past.tolist() == [n + new for n in lens]
-    u, e = half_step(BF), 2.0 ** -14
+    u = half_step(BF)
     for b, n in enumerate(lens):
         qk = hip.rope_axes(rows[b][:, :(Hq + Hkv) * D], spots[b].to(DEV).contiguous(), rope, Hq + Hkv, D)
         r = wo.attention(qk[:, :Hq * D], qk[:, Hq * D:], rows[b][:, (Hq + Hkv) * D:], [(0, n + new, 0, n + new)], Hq, Hkv, D, left, 0, sinks, D ** -0.5)
-        within(torch.cat(got[b]), r["out"], u * r["out"].abs() + (u + e) * r["out_abs"], "together")
+        within(torch.cat(got[b]), r["out"], u * r["out"].abs() + terms(r, "out", u), "together")
 
 
 def test_captured_training_and_steps_replay():
