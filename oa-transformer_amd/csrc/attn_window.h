@@ -77,12 +77,21 @@ template <int D> OAT_DEV void load_cols(s16x8 (&f)[D / 16], const char* row) {
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) f[ks] = *reinterpret_cast<const s16x8*>(row + (2 * ks + half) * 16);
 }
+// maximum / sum of a value over lanes l and l ^ 32 (one register swap of the halves, no LDS)
 OAT_DEV float both_halves(float v, bool max) {
-  const float o = __shfl_xor(v, 32, 64);
-  return max ? fmaxf(v, o) : v + o;
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+  const float x = __builtin_bit_cast(float, (int)r[0]), y = __builtin_bit_cast(float, (int)r[1]);
+  return max ? fmaxf(x, y) : x + y;
 }
-// every wave's copies have landed and every wave is done reading what the next copies overwrite
-OAT_DEV void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// every wave's copies have landed and every wave is done reading what the next copies overwrite.  The wait is the builtin (vmcnt 0,
+// lgkmcnt 0), not asm: the compiler then knows that its own earlier loads are done and puts no wait for them into the loop, which
+// would wait for the next tile's copies too.
+OAT_DEV void tile_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // ---- sequences and visibility.  Query i of a sequence stands at position p = i + nk - nq (its last query at its last key); it sees
 // key j if  j <= p + right  and  (j >= p - left  or  j < sinks).
@@ -118,6 +127,15 @@ OAT_DEV bool place(int tiles, int heads, int B, Place& p) {
 }
 inline unsigned place_grid(long long n) { return (unsigned)((n + 7) / 8 * 8); }
 
+// The visibility of the pair that register r of a C fragment holds, with the fixed side (a query's keys lo .. hi and sinks, or a key's
+// queries) folded into bounds on the register's row number: row <= hi and (row >= lo or row < sink), no branches.
+struct Bounds {
+  int lo, hi, sink;
+  OAT_DEV bool sees(int r) const {
+    const int row = 8 * (r >> 2) + (r & 3);
+    return (row <= hi) & ((row >= lo) | (row < sink));
+  }
+};
 // the key tiles (of 64) that queries at positions p0 .. p1 see: those of the sinks, then those of the window
 struct KeyTiles {
   int sink, first, count;

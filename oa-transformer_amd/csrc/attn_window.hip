@@ -9,7 +9,7 @@ namespace oat {
 // The query is the COLUMN of S^T: a lane holds 16 of 32 keys of ONE query, so maximum and sum of a row are register work and one
 // exchange with lane ^ 32, and P^T is the B operand of the second product where it stands.
 template <class T, int D>
-__global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TB];         // K, V x 2
   const int tiles = (a.max_q + 127) / 128;
@@ -60,12 +60,12 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
     }
     if (!full) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        const int jb = j0 + u * 32 + 4 * half;
+        const Bounds bd{lo - jb, hi - jb, a.sinks - jb};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + u * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (!(j <= hi && (j >= lo || j < a.sinks))) st[u][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r) st[u][r] = bd.sees(r) ? st[u][r] : -INFINITY;
+      }
     }
     float mx = st[0][0];
 #pragma unroll
@@ -73,9 +73,10 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[u][r]);
     const float mn = fmaxf(m, both_halves(mx, true));
-    const float mc = mn == -INFINITY ? 0.f : mn * c;
-    if (__any(mn > m)) {
-      const float al = __builtin_amdgcn_exp2f(m * c - mc);
+    // the reference maximum moves only when a row's own has grown by more than 2^6: until then its terms are at most 2^6 (64), which
+    // costs no precision, and the sums need no rescaling
+    if (__any((mn - m) * c > 6.f)) {
+      const float al = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.f : mn)) * c);
       l *= al;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -83,6 +84,7 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
         for (int r = 0; r < 16; ++r) o[dt][r] *= al;
       m = mn;
     }
+    const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a) {
 
 // dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
 template <class T, int D>
-__global__ __launch_bounds__(256) void win_bwd_q_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
   const int tiles = (a.max_q + 127) / 128;
@@ -201,11 +203,10 @@ __global__ __launch_bounds__(256) void win_bwd_q_kernel(WinArgs a) {
         st[r] = pr * (dp[r] - delta);
       }
       if (!full) {
+        const int jb = j0 + u * 32 + 4 * half;
+        const Bounds bd{lo - jb, hi - jb, a.sinks - jb};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + u * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (!(j <= hi && (j >= lo || j < a.sinks))) st[r] = 0.f;
-        }
+        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(256) void win_bwd_q_kernel(WinArgs a) {
 // dK and dV of 128 keys (32 a wave): S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and
 // their gradients pass through the LDS in tiles of 64, with their lse2 and delta
 template <class T, int D>
-__global__ __launch_bounds__(256) void win_bwd_kv_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   __shared__ __attribute__((aligned(1024))) char lds[2 * ST];
   const int tiles = (a.max_k + 127) / 128;
@@ -310,11 +311,9 @@ __global__ __launch_bounds__(256) void win_bwd_kv_kernel(WinArgs a) {
         }
       }
       if (iu < flo || iu + 31 > fhi) {
+        const Bounds bd{ilo - iu - 4 * half, ihi - iu - 4 * half, 0};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = iu + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (!(i >= ilo && i <= ihi)) st[r] = 0.f;
-        }
+        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] *= st[r];
