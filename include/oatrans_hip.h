@@ -310,7 +310,7 @@ int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dt
 int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
                         float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
                         int left, int right, int sinks, float scale, void* stream);
-size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int Hq);
+size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max_q, int max_k, int Hq, int Hkv, int D, int left, int sinks);
 /* dq, dk, dv of the same call (written, not accumulated; fixed order of every sum).  Sequences must not share query or key rows. */
 int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out, long long ldo,
                         const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk, long long lddk, void* dv,

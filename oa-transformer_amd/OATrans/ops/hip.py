@@ -39,7 +39,7 @@ _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_
 _WINDOW_SIGNATURES = {
     "oat_rope_axes": (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _I, _I, ctypes.POINTER(_OatRope), _I, _P]),
     "oat_attn_window_fwd": (_I, [_P, _L] * 4 + [_P, _P] + [_I] * 12 + [_F, _P]),
-    "oat_attn_window_bwd_workspace_bytes": (_Z, [_I, _I]),
+    "oat_attn_window_bwd_workspace_bytes": (_Z, [_I] * 9),
     "oat_attn_window_bwd": (_I, [_P, _L] * 4 + [_P] + [_P, _L] * 4 + [_P] + [_I] * 12 + [_F, _P, _Z, _P]),
     "oat_attn_window_step_workspace_bytes": (_Z, [_I] * 4),
     "oat_attn_window_step": (_I, [_P, _L, _P, _P, _P, ctypes.POINTER(_L), _I, _P, _L] + [_I] * 8 + [_F, ctypes.POINTER(_OatRope), _P, _P, _Z, _P]),
@@ -1118,7 +1118,7 @@ def attn_window_fwd(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, left
 def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, max_q, max_k, left=-1, right=0, sinks=0, scale=None,
                     dq=None, dk=None, dv=None, workspace=None):
     """(dq, dk, dv) of attn_window_fwd.  New outputs start as zeros, given ones keep their rows of no sequence.  workspace: fp32 of
-    oat_attn_window_bwd_workspace_bytes(rows, heads) bytes (default: a new one)."""
+    oat_attn_window_bwd_workspace_bytes(...) bytes (default: a new one)."""
     what = "attn_window_bwd"
     _window_args(q, k, v, seqs, heads, kv_heads, head_dim, what)
     D, dt, dev, M = head_dim, q.dtype, q.device, q.shape[0]
@@ -1135,7 +1135,7 @@ def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, ma
     _rows(dv, kv_heads * D, dt, dev, what + ": dv")
     _need(dq.shape[0] == M and dk.shape[0] == dv.shape[0] == k.shape[0], what + ": dq, dk, dv have as many rows as q, k, v")
     if workspace is None:
-        workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, heads) // 4, dtype=torch.float32, device=dev)
+        workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, seqs.shape[0], max_q, max_k, heads, kv_heads, D, left, sinks) // 4, dtype=torch.float32, device=dev)
     _need(workspace.is_contiguous() and workspace.device == dev, what + ": workspace must be contiguous on the same device")
     _launch(dev, lambda s: lib().oat_attn_window_bwd(
         q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr(), dout.data_ptr(), _ld(dout),

@@ -102,7 +102,9 @@ struct WinArgs {
   float *lse2, *delta;                  // backward: [Hq, rows_q], base 2; sum of dout * out
   long long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;      // bytes
   const int4* seqs;                     // first query row, queries, first key row, keys
+  float* slabs;                         // backward: the sinks' sums (win_bwd_kv_kernel)
   int B, Hq, Hkv, left, right, sinks, max_q, max_k, rows_q, rows_k;
+  int groups, pieces;                   // how the sinks' far queries are split
   float scale;
 };
 struct Seq { int q0, nq, k0, nk; };

@@ -231,25 +231,40 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
 }
 
 // dK and dV of 128 keys (32 a wave): S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and
-// their gradients pass through the LDS in tiles of 64, with their lse2 and delta
-template <class T, int D>
+// their gradients pass through the LDS in tiles of 64, with their lse2 and delta.
+//
+// The sinks' keys are seen by every later query: one workgroup would walk the whole sequence while the others walk a window.  So the
+// pairs beyond the window (the far ones) get workgroups of their own: 32 sink keys and one of `pieces` shares of the far queries each,
+// where waves 0, 1 form dV and waves 2, 3 dK of the tile's two halves.  Those sums, and what the window gives the sinks, go to 32-bit
+// slabs that win_bwd_sink_kernel adds in a fixed order.
+template <class T, int D, bool far>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   __shared__ __attribute__((aligned(1024))) char lds[2 * ST];
-  const int tiles = (a.max_k + 127) / 128;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
   Place pl;
-  if (!place(tiles, a.Hkv, a.B, pl)) return;
+  int piece = 0, group = 0;
+  if constexpr (far) {
+    const int i = blockIdx.x;
+    if (i >= a.B * a.Hkv * a.groups * a.pieces) return;
+    piece = i % a.pieces;
+    group = i / a.pieces % a.groups;
+    pl.h = i / a.pieces / a.groups % a.Hkv;
+    pl.b = i / a.pieces / a.groups / a.Hkv;
+  } else {
+    if (!place((a.max_k + 127) / 128, a.Hkv, a.B, pl)) return;
+  }
   const Seq s = load_seq(a, pl.b);
-  const int j0 = pl.tile * 128;
-  if (j0 >= s.nk) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int off = s.nk - s.nq, G = a.Hq / a.Hkv;
-  // queries that see any of these keys
-  auto first_q = [&](int j) { return max(0, j - a.right - off); };
-  auto last_q = [&](int jl, int jh) { return jl < a.sinks ? s.nq - 1 : min(s.nq - 1, jh + a.left - off); };
-  const int jend = min(j0 + 127, s.nk - 1);
-  const int t0 = first_q(j0) / TILE, t1 = last_q(j0, jend) < first_q(j0) ? t0 - 1 : last_q(j0, jend) / TILE;
-  const int nt = max(0, t1 - t0 + 1), count = nt * G;
+  const int j0 = far ? group * 32 : pl.tile * 128;
+  if (j0 >= s.nk || (far && j0 >= a.sinks)) return;
+  const int off = s.nk - s.nq, split = a.groups > 0;
+  // the queries that see key j: i = lo(j) .. hi(j)
+  auto lo = [&](int j) { return far ? j + a.left - off + 1 : j - a.right - off; };
+  auto hi = [&](int j) { return far ? (j < a.sinks ? s.nq - 1 : -1) : !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
+  const int jend = min(j0 + (far ? 31 : 127), s.nk - 1);
+  const int i0 = max(0, lo(j0)), i1 = far || (!split && j0 < a.sinks) ? s.nq - 1 : hi(jend);
+  const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1;
+  const int na = far ? (int)((long long)nt * G * piece / a.pieces) : 0, nb = far ? (int)((long long)nt * G * (piece + 1) / a.pieces) : nt * G;
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
   auto stage = [&](int n) {
     const int g = n / nt, i0 = (t0 + n - g * nt) * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
@@ -265,24 +280,26 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
                    : "=&s"(keep) : "v"((uint32_t)min(lane, last) * 4u), "s"(src), "s"(dst) : "memory");
     }
   };
-  const int jw = j0 + wave * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1);
-  const int jwe = min(jw + 31, s.nk - 1);
+  const int jw = far ? j0 : j0 + wave * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1), jwe = min(jw + 31, s.nk - 1);
   const float c = a.scale * LOG2E;
   s16x8 kf[D / 16], vf[D / 16];
   load_cols<D>(kf, a.k + (long long)(s.k0 + jc) * a.ldk + pl.h * (D * 2));
   load_cols<D>(vf, a.v + (long long)(s.k0 + jc) * a.ldv + pl.h * (D * 2));
-  const int ilo = j - a.right - off, ihi = j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off);   // this key's queries
-  const int wlo = first_q(jw), whi = last_q(jw, jwe);                                                  // those of any key of the wave
-  const int flo = jwe - a.right - off, fhi = jwe < a.sinks ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);   // those of every key
+  const int ilo = lo(j), ihi = j < s.nk ? hi(j) : -1;
+  const bool sink_w = jwe < a.sinks;                                    // the wave's keys are sinks all
+  // queries wlo .. whi see a key of the wave, flo .. fhi see them all
+  const int wlo = lo(jw), whi = far || (!split && jw < a.sinks) ? s.nq - 1 : hi(jwe);
+  const int flo = lo(jwe), fhi = far ? (sink_w ? s.nq - 1 : -1) : !split && sink_w ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);
+  const bool do_k = !far || wave >= 2, do_v = !far || wave < 2;
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
-  if (count) stage(0);
-  for (int n = 0; n < count; ++n) {
+  if (na < nb) stage(na);
+  for (int n = na; n < nb; ++n) {
     tile_barrier();
-    if (n + 1 < count) stage(n + 1);
+    if (n + 1 < nb) stage(n + 1);
     const int it = (t0 + n % nt) * TILE;
     const char* Qt = lds + (n & 1) * ST;
     const char* Dt = Qt + TB;
@@ -290,14 +307,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int iu = it + u * 32;
-      if (jw >= s.nk || iu > whi || iu + 31 < wlo) continue;
+      if (jw >= s.nk || iu > whi || iu + 31 < wlo || (far && u != (wave & 1))) continue;
       f32x16 st, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
-        dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
+      for (int ks = 0; ks < D / 16; ++ks) st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
+      if (do_k) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -315,18 +333,39 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
       }
+      if (do_v) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] *= st[r];
+        for (int h = 0; h < 2; ++h) {
+          const s16x8 pf = pack8<T>(st, h);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const s16x8 pf = pack8<T>(st, h), sf = pack8<T>(dp, h);
+          for (int dt = 0; dt < D / 32; ++dt) dv[dt] = mfma32<T>(col_frag32<D>(Dt, u * 32 + h * 16, dt), pf, dv[dt]);
+        }
+      }
+      if (do_k) {
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          dv[dt] = mfma32<T>(col_frag32<D>(Dt, u * 32 + h * 16, dt), pf, dv[dt]);
-          dk[dt] = mfma32<T>(col_frag32<D>(Qt, u * 32 + h * 16, dt), sf, dk[dt]);
+        for (int r = 0; r < 16; ++r) dp[r] *= st[r];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const s16x8 sf = pack8<T>(dp, h);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) dk[dt] = mfma32<T>(col_frag32<D>(Qt, u * 32 + h * 16, dt), sf, dk[dt]);
         }
       }
     }
+  }
+  if (far || (split && jw < a.sinks)) {
+    // [slot][dK, dV][D][32 keys]; slots: (piece, half of its tiles), last the window's own
+    const int slots = 2 * a.pieces + 1, slot = far ? 2 * piece + (wave & 1) : slots - 1, gi = far ? group : jw / 32;
+    float* sl = a.slabs + (((size_t)(pl.b * a.Hkv + pl.h) * a.groups + gi) * slots + slot) * (2 * D * 32) + (lane & 31);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (do_k) sl[d * 32] = dk[dt][r];
+        if (do_v) sl[(D + d) * 32] = dv[dt][r];
+      }
+    return;
   }
   if (j >= s.nk) return;
   char* pk = a.dk + (long long)(s.k0 + j) * a.lddk + pl.h * (D * 2);
@@ -342,6 +381,47 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
       *reinterpret_cast<T4*>(pk + (dt * 32 + 8 * g + 4 * half) * 2) = x;
       *reinterpret_cast<T4*>(pv + (dt * 32 + 8 * g + 4 * half) * 2) = y;
     }
+}
+
+// the sinks' slabs, added slot by slot: a thread = one key, 8 values of dK or dV
+template <class T, int D>
+__global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
+  const int key = threadIdx.x & 31, d8 = blockIdx.y * 8 + (threadIdx.x >> 5);          // d8: 0 .. 2 D / 8
+  const int group = blockIdx.x % a.groups, h = blockIdx.x / a.groups % a.Hkv, b = blockIdx.x / a.groups / a.Hkv;
+  const Seq s = load_seq(a, b);
+  const int j = group * 32 + key;
+  if (group * 32 >= a.sinks || j >= s.nk) return;
+  const int slots = 2 * a.pieces + 1;
+  const float* sl = a.slabs + ((size_t)blockIdx.x * slots) * (2 * D * 32) + d8 * 8 * 32 + key;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < slots; ++i, sl += 2 * D * 32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += sl[e * 32];
+  }
+  const bool is_v = d8 >= D / 8;
+  typedef __attribute__((ext_vector_type(8))) T T8;
+  T8 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = (T)(is_v ? x[e] : x[e] * a.scale);
+  char* p = is_v ? a.dv + (long long)(s.k0 + j) * a.lddv : a.dk + (long long)(s.k0 + j) * a.lddk;
+  *reinterpret_cast<T8*>(p + h * (D * 2) + (is_v ? d8 - D / 8 : d8) * 16) = y;
+}
+
+// how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries; 0 groups: the sinks' own tiles walk all
+// queries.  That takes max_q / 64 steps where a window's tile takes (left + right + 128) / 64: split where it is over 512 queries longer.
+struct FarSplit { int groups, pieces; };
+static FarSplit far_split(int B, int Hq, int Hkv, int max_q, int max_k, int left, int sinks) {
+  const long long rows = min((long long)max_q, (long long)max_k - left);
+  if (sinks < 1 || rows <= 512 || B < 1) return {0, 0};
+  const int groups = (min(sinks, max_k) + 31) / 32;
+  const long long want = 512 / max(1ll, (long long)B * Hkv * groups);
+  return {groups, (int)max(1ll, min(want, rows * (Hq / Hkv) / 256))};
+}
+static size_t slab_floats(const FarSplit& f, int B, int Hkv, int D) {
+  return (size_t)B * Hkv * f.groups * (2 * f.pieces + 1) * 2 * D * 32;
 }
 
 static bool rows_wrong(const void* p, long long ld, int heads, int D) {
@@ -371,13 +451,19 @@ static int far(int n) { return n < 0 || n > (1 << 29) ? 1 << 29 : n; }      // a
 
 using namespace oat;
 
-#define WIN_LAUNCH(kernel, blocks)                                                                                   \
+#define WIN_FWD(T, D) win_fwd_kernel<T, D>
+#define WIN_Q(T, D) win_bwd_q_kernel<T, D>
+#define WIN_FAR(T, D) win_bwd_kv_kernel<T, D, true>
+#define WIN_KV(T, D) win_bwd_kv_kernel<T, D, false>
+#define WIN_SINK(T, D) win_bwd_sink_kernel<T, D>
+#define WIN_LAUNCH(kernel, blocks) WIN_LAUNCH2(kernel, dim3(place_grid(blocks)))
+#define WIN_LAUNCH2(kernel, grid)                                                                                    \
   do {                                                                                                               \
-    const dim3 g_(place_grid(blocks));                                                                               \
-    if (dtype == 0 && D == 64) OAT_LAUNCH(kernel<bf16, 64>, g_, dim3(256), 0, s, a);                                 \
-    else if (dtype == 0) OAT_LAUNCH(kernel<bf16, 128>, g_, dim3(256), 0, s, a);                                      \
-    else if (D == 64) OAT_LAUNCH(kernel<_Float16, 64>, g_, dim3(256), 0, s, a);                                      \
-    else OAT_LAUNCH(kernel<_Float16, 128>, g_, dim3(256), 0, s, a);                                                  \
+    const dim3 g_ = (grid);                                                                                          \
+    if (dtype == 0 && D == 64) OAT_LAUNCH((kernel(bf16, 64)), g_, dim3(256), 0, s, a);                                 \
+    else if (dtype == 0) OAT_LAUNCH((kernel(bf16, 128)), g_, dim3(256), 0, s, a);                                      \
+    else if (D == 64) OAT_LAUNCH((kernel(_Float16, 64)), g_, dim3(256), 0, s, a);                                      \
+    else OAT_LAUNCH((kernel(_Float16, 128)), g_, dim3(256), 0, s, a);                                                  \
   } while (0)
 
 extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
@@ -396,11 +482,14 @@ extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  WIN_LAUNCH(win_fwd_kernel, (long long)B * Hq * ((max_q + 127) / 128));
+  WIN_LAUNCH(WIN_FWD, (long long)B * Hq * ((max_q + 127) / 128));
   return check_launch("attn_window_fwd");
 }
 
-extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int Hq) { return (size_t)rows_q * Hq * 8; }
+extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max_q, int max_k, int Hq, int Hkv, int D, int left, int sinks) {
+  if (rows_q < 0 || Hq < 1 || Hkv < 1 || D < 1) return 0;
+  return ((size_t)rows_q * Hq * 2 + slab_floats(far_split(B, Hq, Hkv, max_q, max_k, far(left), sinks), B, Hkv, D)) * 4;
+}
 
 extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
                                    long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
@@ -417,7 +506,7 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
     set_error("attn_window_bwd: k, v, dk, dv need 16-byte aligned rows (pitch a multiple of 8, at least the heads, at most 2^22 values)");
     return -2;
   }
-  if (rows_q && (!workspace || workspace_bytes < oat_attn_window_bwd_workspace_bytes(rows_q, Hq))) { set_error("attn_window_bwd: the workspace is too small"); return -3; }
+  if (rows_q && (!workspace || workspace_bytes < oat_attn_window_bwd_workspace_bytes(rows_q, B, max_q, max_k, Hq, Hkv, D, left, sinks))) { set_error("attn_window_bwd: the workspace is too small"); return -3; }
   WinArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.dout = (const char*)dout;
   a.lse = const_cast<float*>(lse); a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;
@@ -427,7 +516,13 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  if (max_q && rows_q) WIN_LAUNCH(win_bwd_q_kernel, (long long)B * Hq * ((max_q + 127) / 128));
-  if (max_k && rows_k) WIN_LAUNCH(win_bwd_kv_kernel, (long long)B * Hkv * ((max_k + 127) / 128));
+  if (max_q && rows_q) WIN_LAUNCH(WIN_Q, (long long)B * Hq * ((max_q + 127) / 128));
+  const FarSplit f = rows_q ? far_split(B, Hq, Hkv, max_q, max_k, a.left, sinks) : FarSplit{0, 0};
+  a.groups = f.groups;
+  a.pieces = f.pieces;
+  a.slabs = a.delta + (size_t)rows_q * Hq;
+  if (max_k && rows_k && f.groups) WIN_LAUNCH(WIN_FAR, (long long)B * Hkv * f.groups * f.pieces);
+  if (max_k && rows_k) WIN_LAUNCH(WIN_KV, (long long)B * Hkv * ((max_k + 127) / 128));
+  if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 64));
   return check_launch("attn_window_bwd");
 }

@@ -79,7 +79,7 @@ def test_attention_backward_needs_its_workspace_and_gradients():
     hip = _hip()
     bwd = lambda lse=4096, dout=4096, dq=4096, ws=4096, n=160: hip.lib().oat_attn_window_bwd(
         4096, 128, 4096, 64, 4096, 64, 4096, 128, lse, dout, 128, dq, 128, 4096, 64, 4096, 64, 4096, 1, 10, 10, 10, 10, 2, 1, 64, 0, -1, 0, 0, 0.125, ws, n, None)
-    need = hip.lib().oat_attn_window_bwd_workspace_bytes(10, 2)
+    need = hip.lib().oat_attn_window_bwd_workspace_bytes(10, 1, 10, 10, 2, 1, 64, -1, 0)
     assert need == 160
     _refused(hip, bwd(n=need - 1), b"workspace")
     _refused(hip, bwd(ws=None), b"workspace")

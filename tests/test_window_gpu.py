@@ -112,6 +112,8 @@ ATTN = [
     ([1100], None, 1, 1, 64, -1, -1, 0),
     ([2300], None, 1, 1, 64, 90, 0, 130),                                             # more sinks than a tile of keys
     ([1500, 1], None, 2, 1, 128, 50, 50, 1),
+    ([1300, 700], None, 4, 1, 128, 100, 0, 40),                                       # the sinks' far queries are split over workgroups
+    ([900, 20], [1400, 900], 4, 2, 64, 60, 10, 3),
 ]
 
 
