@@ -16,6 +16,8 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
+#define WIN_INLINE __attribute__((always_inline))
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 template <class T> OAT_DEV f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c);
@@ -41,17 +43,34 @@ template <int D> OAT_DEV int swz(int r) { return (D == 64 ? ((r >> 1) & 1) << 2 
 
 constexpr int TILE = 64;
 
-// asynchronous copy of a tile by 256 threads: rows 0 .. TILE - 1 from `base` (wave-uniform), pitch `ldb` bytes; rows past `last`
-// repeat that row, so that no memory outside the sequence is read and nothing but its own finite values stands in the tile
-template <int D> OAT_DEV void stage_tile(const char* base, uint32_t ldb, int last, uint32_t lds) {
-  constexpr int CPR = D / 8;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-#pragma unroll
-  for (int i = 0; i < TILE * CPR / 256; ++i) {
-    const int c = i * 256 + tid, r = c / CPR, ch = (c % CPR) ^ swz<D>(r);
-    glds16_asm_lds(base, (uint32_t)min(r, last) * ldb + ch * 16, lds + (i * 256 + wave * 64) * 16);
+// Asynchronous copies of tiles by 256 threads: rows 0 .. TILE - 1 from `base` (wave-uniform), pitch `ldb` bytes.  A whole tile takes one
+// lane offset for all of its pieces (a piece is 256 / CPR rows, and swz repeats with them): no vector instructions.  In a ragged tile the
+// rows past `last` repeat that row, so that no memory outside the sequence is read and nothing but its own finite values stands there.
+template <int D> struct Stager {
+  static constexpr int CPR = D / 8, RPP = 256 / CPR;                   // chunks of a row, rows of a piece
+  uint32_t ldb, off, wave;
+  OAT_DEV Stager(long long ld) {
+    const int tid = threadIdx.x, r = tid / CPR;
+    ldb = (uint32_t)ld;
+    off = r * ldb + (((tid % CPR) ^ swz<D>(r)) << 4);
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
   }
-}
+  OAT_DEV void operator()(const char* base, int last, uint32_t lds) const {
+    lds += wave;
+    if (last >= TILE - 1) {
+#pragma unroll
+      for (int i = 0; i < TILE / RPP; ++i) glds16(base + (size_t)i * RPP * ldb, off, lds + i * 4096);
+    } else {
+      const int tid = threadIdx.x, r0 = tid / CPR;
+      const uint32_t ch = ((tid % CPR) ^ swz<D>(r0)) << 4;
+#pragma unroll
+      for (int i = 0; i < TILE / RPP; ++i) glds16(base, (uint32_t)min(i * RPP + r0, last) * ldb + ch, lds + i * 4096);
+    }
+  }
+  OAT_DEV static void glds16(const char* base, uint32_t lane_off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
+  }
+};
 // A fragment: rows rb .. rb + 31 of a tile, k = 16 ks .. +16
 template <int D> OAT_DEV s16x8 row_frag32(const char* tile, int rb, int ks) {
   const int lane = threadIdx.x & 63, r = lane & 31;
@@ -138,6 +157,22 @@ struct Bounds {
     return (row <= hi) & ((row >= lo) | (row < sink));
   }
 };
+// masks the scores of 32 keys (the first at jb for this lane's half; lo .. hi and the sinks are what its query sees).  Most tiles that
+// are not seen whole lie across one edge only: one comparison each.
+template <bool ZERO> OAT_DEV void mask_keys(f32x16& S, int jb, int lo, int hi, int sinks, bool edge_lo, bool edge_hi) {
+  const float no = ZERO ? 0.f : -INFINITY;
+  const Bounds bd{lo - jb, hi - jb, sinks - jb};
+  if (!edge_lo) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) <= bd.hi ? S[r] : no;
+  } else if (!edge_hi && sinks <= jb) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) >= bd.lo ? S[r] : no;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[r] = bd.sees(r) ? S[r] : no;
+  }
+}
 // the key tiles (of 64) that queries at positions p0 .. p1 see: those of the sinks, then those of the window
 struct KeyTiles {
   int sink, first, count;

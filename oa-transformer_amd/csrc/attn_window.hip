@@ -11,7 +11,7 @@ namespace oat {
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TB];         // K, V x 2
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TB];         // K x 2, V x 2
   const int tiles = (a.max_q + 127) / 128;
   Place pl;
   if (!place(tiles, a.Hq, a.B, pl)) return;
@@ -24,10 +24,14 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   const char* kb = a.k + (long long)s.k0 * a.ldk + hk * (D * 2);
   const char* vb = a.v + (long long)s.k0 * a.ldv + hk * (D * 2);
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
-  auto stage = [&](int n) {
+  const Stager<D> sk(a.ldk), sv(a.ldv);
+  auto stage_k = [&](int n, int buf) WIN_INLINE {
     const int j0 = kt.at(n) * TILE;
-    stage_tile<D>(kb + (long long)j0 * a.ldk, (uint32_t)a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
-    stage_tile<D>(vb + (long long)j0 * a.ldv, (uint32_t)a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
+    sk(kb + (long long)j0 * a.ldk, s.nk - 1 - j0, l0 + buf * TB);
+  };
+  auto stage_v = [&](int n, int buf) WIN_INLINE {
+    const int j0 = kt.at(n) * TILE;
+    sv(vb + (long long)j0 * a.ldv, s.nk - 1 - j0, l0 + (2 + buf) * TB);
   };
   const int iw = i0 + wave * 32, i = iw + (lane & 31), ic = min(i, s.nq - 1);
   const int p = ic + off, hi = min(s.nk - 1, p + a.right), lo = p - a.left;
@@ -35,72 +39,146 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   const float c = a.scale * LOG2E;
   s16x8 qf[D / 16];
   load_cols<D>(qf, a.q + (long long)(s.q0 + ic) * a.ldq + pl.h * (D * 2));
-  f32x16 o[D / 32];
+  f32x16 o[D / 32], S0, S1;
+  s16x8 P0[2], P1[2];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  if (kt.count) stage(0);
-  for (int n = 0; n < kt.count; ++n) {
-    tile_barrier();
-    if (n + 1 < kt.count) stage(n + 1);
-    const int j0 = kt.at(n) * TILE;
-    if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) continue;
-    const bool full = j0 + TILE - 1 <= min(s.nk - 1, wp0 + a.right) && (j0 >= wp1 - a.left || j0 + TILE - 1 < a.sinks);
-    const char* Kt = lds + (n & 1) * 2 * TB;
-    const char* Vt = Kt + TB;
-    f32x16 st[2];
+  // probabilities are formed relative to a reference score m of the row, 2^(c s + neg), neg = -c m
+  float neg = 0.f, l = 0.f;
+  bool begun = false, all_begun = false;                               // the row has a reference; every row of the wave has
+  auto scores = [&](const char* K, int u, f32x16& S) WIN_INLINE {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int r = 0; r < 16; ++r) S[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[u][r] = 0.f;
+    for (int ks = 0; ks < D / 16; ++ks) S = mfma32<T>(row_frag32<D>(K, u * 32, ks), qf[ks], S);
+  };
+  auto values = [&](const char* V, int u, const s16x8 (&P)[2]) WIN_INLINE {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) st[u] = mfma32<T>(row_frag32<D>(Kt, u * 32, ks), qf[ks], st[u]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma32<T>(col_frag32<D>(V, u * 32 + h * 16, dt), P[h], o[dt]);
+  };
+  auto row_max = [&](const f32x16& S) WIN_INLINE {
+    float mx = S[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
+    return both_halves(mx, true);
+  };
+  auto exponentials = [&](const f32x16& S, s16x8 (&P)[2]) WIN_INLINE {
+    f32x16 E;
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      E[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], c, neg));
+      t += E[r];
     }
-    if (!full) {
+    P[0] = pack8<T>(E, 0);
+    P[1] = pack8<T>(E, 1);
+    return t;
+  };
+  // One step = 32 keys: their exponentials (vector unit) beside the products of the 32 before (values) and after (scores), which do not
+  // depend on them.  The scheduling groups deal the products out over the exponentials: one unit would wait for the other otherwise.
+  // The reference is the maximum of the first keys a row sees, not a running one (a third of the vector work): it moves only when a sum
+  // of 16 terms passes 2^10 - then the step's terms are formed again - and until then no term is over 2^10, which costs no precision.
+  auto step = [&](int n, int u, const f32x16& S_, s16x8 (&P)[2], const char* V, const s16x8 (&Pv)[2], const char* K, f32x16& Sq) WIN_INLINE {
+    f32x16 S = S_;
+    s16x8 kf[D / 16], vf[2][D / 32];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int jb = j0 + u * 32 + 4 * half;
-        const Bounds bd{lo - jb, hi - jb, a.sinks - jb};
+    for (int ks = 0; ks < D / 16; ++ks) kf[ks] = row_frag32<D>(K, (1 - u) * 32, ks);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[u][r] = bd.sees(r) ? st[u][r] : -INFINITY;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) vf[h][dt] = col_frag32<D>(V, (1 - u) * 32 + h * 16, dt);
+    const int j0 = kt.at(n) * TILE + u * 32;
+    const bool edge_hi = j0 + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = j0 < wp1 - a.left && j0 + 31 >= a.sinks;
+    if (edge_lo | edge_hi) mask_keys<false>(S, j0 + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
+    if (!all_begun) {
+      const float mx = row_max(S);
+      if (!begun && mx > -INFINITY) {
+        neg = -mx * c;
+        begun = true;
       }
+      all_begun = __all(begun);
     }
-    float mx = st[0][0];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int r = 0; r < 16; ++r) Sq[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[u][r]);
-    const float mn = fmaxf(m, both_halves(mx, true));
-    // the reference maximum moves only when a row's own has grown by more than 2^6: until then its terms are at most 2^6 (64), which
-    // costs no precision, and the sums need no rescaling
-    if (__any((mn - m) * c > 6.f)) {
-      const float al = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.f : mn)) * c);
+    for (int ks = 0; ks < D / 16; ++ks) {
+      Sq = mfma32<T>(kf[ks], qf[ks], Sq);
+      const int h = ks / (D / 32), dt = ks % (D / 32);
+      o[dt] = mfma32<T>(vf[h][dt], Pv[h], o[dt]);
+    }
+    float t = exponentials(S, P);
+    asm volatile("" : "+v"(P[0]), "+v"(P[1]), "+v"(t));                // formed here, not where they are next read
+#pragma unroll
+    for (int k = 0; k < D / 8; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);               // a matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x002, 64 / (D / 8), 0);    // vector instructions
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(t > 1024.f)) {
+      const float to = fminf(neg, -row_max(S) * c);                    // (a row that sees nothing here: +inf, the minimum stays)
+      float al = __builtin_amdgcn_exp2f(begun ? to - neg : 0.f);
+      if (begun) neg = to;
+      asm volatile("" : "+v"(al));                                     // (nothing of this before the branch)
       l *= al;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= al;
-      m = mn;
+      t = exponentials(S, P);
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        st[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[u][r], c, -mc));
-        l += st[u][r];
-      }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const s16x8 pf = pack8<T>(st[u], h);
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma32<T>(col_frag32<D>(Vt, u * 32 + h * 16, dt), pf, o[dt]);
-      }
+    l += t;
+  };
+  // K of tiles n, n + 1 and V of tiles n - 1, n are in use at tile n, so the next copies start between its two steps
+  P1[0] = P1[1] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  if (kt.count) {
+    stage_k(0, 0);
+    stage_v(0, 0);
+    stage_v(0, 1);                                                     // (what the first step multiplies by zeros has to be numbers)
   }
+  tile_barrier();
+  if (kt.count > 1) stage_k(1, 1);
+  auto turn = [&](int n, int odd) WIN_INLINE {                                    // between a tile's two steps
+    tile_barrier();
+    if (n + 2 < kt.count) stage_k(n + 2, odd);
+    if (n + 1 < kt.count) stage_v(n + 1, 1 - odd);
+  };
+  // (where tile n + 1 does not exist, its scores are formed from what stands there and not used)
+  auto tile = [&](int n, int odd) WIN_INLINE {
+    const char *K0 = lds + odd * TB, *K1 = lds + (1 - odd) * TB, *V0 = lds + (3 - odd) * TB, *V1 = lds + (2 + odd) * TB;
+    step(n, 0, S0, P0, V0, P1, K0, S1);
+    turn(n, odd);
+    step(n, 1, S1, P1, V1, P0, K1, S0);
+  };
+  // the wave's own tiles na .. nb - 1 of the list (those between that only other waves see are masked).  The loop has no branch around
+  // the sums - where paths with and without products meet, the compiler copies all of o - and two tiles a turn, so that all LDS
+  // addresses are constants.
+  const int hw = iw < s.nq ? min(s.nk - 1, wp1 + a.right) : -1, ht = hw / TILE;
+  const int nb = hw < 0 ? 0 : ht < kt.sink ? ht + 1 : max(kt.sink, ht - kt.first + kt.sink + 1);
+  const int na = kt.sink ? 0 : min(nb, max(0, max(0, wp0 - a.left) / TILE - kt.first));
+  int n = 0;
+  for (; n < na; ++n) turn(n, n & 1);
+  if (n < nb) {
+    scores(lds + (n & 1) * TB, 0, S0);
+    if (n & 1) {
+      tile(n, 1);
+      ++n;
+    }
+    for (; n + 1 < nb; n += 2) {
+      tile(n, 0);
+      tile(n + 1, 1);
+    }
+    if (n < nb) {
+      tile(n, 0);
+      ++n;
+    }
+    values(lds + (2 + ((n - 1) & 1)) * TB, 1, P1);
+  }
+  for (; n < kt.count; ++n) turn(n, n & 1);
   if (i >= s.nq) return;
   l = both_halves(l, false);
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -115,7 +193,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
       for (int e = 0; e < 4; ++e) y[e] = (T)(o[dt][4 * g + e] * inv);
       *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = y;
     }
-  if (a.lse && half == 0) a.lse[(size_t)(s.q0 + i) * a.Hq + pl.h] = l > 0.f ? m * a.scale + __logf(l) : -INFINITY;
+  if (a.lse && half == 0) a.lse[(size_t)(s.q0 + i) * a.Hq + pl.h] = l > 0.f ? (__log2f(l) - neg) * LN2 : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------- backward
@@ -141,10 +219,11 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   const char* kb = a.k + (long long)s.k0 * a.ldk + hk * (D * 2);
   const char* vb = a.v + (long long)s.k0 * a.ldv + hk * (D * 2);
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
-  auto stage = [&](int n) {
+  const Stager<D> sk(a.ldk), sv(a.ldv);
+  auto stage = [&](int n) WIN_INLINE {
     const int j0 = kt.at(n) * TILE;
-    stage_tile<D>(kb + (long long)j0 * a.ldk, (uint32_t)a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
-    stage_tile<D>(vb + (long long)j0 * a.ldv, (uint32_t)a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
+    sk(kb + (long long)j0 * a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
+    sv(vb + (long long)j0 * a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
   };
   const int iw = i0 + wave * 32, i = iw + (lane & 31), ic = min(i, s.nq - 1);
   const int p = ic + off, hi = min(s.nk - 1, p + a.right), lo = p - a.left;
@@ -184,7 +263,6 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
     if (n + 1 < kt.count) stage(n + 1);
     const int j0 = kt.at(n) * TILE;
     if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) continue;
-    const bool full = j0 + TILE - 1 <= min(s.nk - 1, wp0 + a.right) && (j0 >= wp1 - a.left || j0 + TILE - 1 < a.sinks);
     const char* Kt = lds + (n & 1) * 2 * TB;
     const char* Vt = Kt + TB;
 #pragma unroll
@@ -202,12 +280,9 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -lse2));
         st[r] = pr * (dp[r] - delta);
       }
-      if (!full) {
-        const int jb = j0 + u * 32 + 4 * half;
-        const Bounds bd{lo - jb, hi - jb, a.sinks - jb};
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
-      }
+      const int ju = j0 + u * 32;
+      const bool edge_hi = ju + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = ju < wp1 - a.left && ju + 31 >= a.sinks;
+      if (edge_lo | edge_hi) mask_keys<true>(st, ju + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const s16x8 sf = pack8<T>(st, h);
@@ -259,19 +334,20 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
   if (j0 >= s.nk || (far && j0 >= a.sinks)) return;
   const int off = s.nk - s.nq, split = a.groups > 0;
   // the queries that see key j: i = lo(j) .. hi(j)
-  auto lo = [&](int j) { return far ? j + a.left - off + 1 : j - a.right - off; };
-  auto hi = [&](int j) { return far ? (j < a.sinks ? s.nq - 1 : -1) : !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
+  auto lo = [&](int j) WIN_INLINE { return far ? j + a.left - off + 1 : j - a.right - off; };
+  auto hi = [&](int j) WIN_INLINE { return far ? (j < a.sinks ? s.nq - 1 : -1) : !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
   const int jend = min(j0 + (far ? 31 : 127), s.nk - 1);
   const int i0 = max(0, lo(j0)), i1 = far || (!split && j0 < a.sinks) ? s.nq - 1 : hi(jend);
   const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1;
   const int na = far ? (int)((long long)nt * G * piece / a.pieces) : 0, nb = far ? (int)((long long)nt * G * (piece + 1) / a.pieces) : nt * G;
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
-  auto stage = [&](int n) {
+  const Stager<D> sq(a.ldq), sd(a.lddo);
+  auto stage = [&](int n) WIN_INLINE {
     const int g = n / nt, i0 = (t0 + n - g * nt) * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
     const long long row = s.q0 + i0;
     const uint32_t l = l0 + (n & 1) * ST;
-    stage_tile<D>(a.q + row * a.ldq + h * (D * 2), (uint32_t)a.ldq, last, l);
-    stage_tile<D>(a.dout + row * a.lddo + h * (D * 2), (uint32_t)a.lddo, last, l + TB);
+    sq(a.q + row * a.ldq + h * (D * 2), last, l);
+    sd(a.dout + row * a.lddo + h * (D * 2), last, l + TB);
     if (wave < 2) {
       const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
       const uint32_t dst = l + 2 * TB + wave * 256;
