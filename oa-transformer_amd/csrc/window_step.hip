@@ -35,11 +35,12 @@ OAT_DEV void put(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED,
 OAT_DEV float get(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 constexpr int SK = 32;                               // keys of a wave's tile
-template <int D> constexpr int step_lds() { return 4 * 2 * 2 * SK * D * 2; }
+template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
 
 // One workgroup = one piece of the visible keys of one (sequence, key head), for up to 16 of the query heads that share it; a wave
-// takes every fourth tile of 32 keys.  Bound: the cache is read once - HBM; so keys and values go straight to the LDS (asynchronous,
-// two tiles of each ahead per wave, no register waits on them) and each wave waits for its own tiles only.  S^T = K Q^T and
+// takes every fourth tile of 32 keys.  Bound: the cache is read once - HBM; so keys and values go straight to the LDS (asynchronous, no
+// register waits on them), a wave waits for its own tiles only, and while it works on a tile's keys its values are on their way (and the
+// next keys while it works on these): 64 KB in flight per CU, with 64 KB of LDS a workgroup (D = 128), so that two or more share a CU.  S^T = K Q^T and
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
 // The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
 // new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in the order of the pieces.
@@ -94,20 +95,21 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
     qs[t] = g < ng ? (T)turned(reinterpret_cast<const T*>(row) + (hk * G + g0 + g) * D, d) : (T)0.f;
   }
   tile_barrier();                                    // the new row has been written before any wave reads it
-  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds) + wave * 4 * TB;
-  char* const mine = lds + wave * 4 * TB;
-  auto stage = [&](int t0, int buf) {
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds) + wave * 2 * TB;
+  const char *Kt = lds + wave * 2 * TB, *Vt = Kt + TB;
+  auto stage = [&](const char* base, long long pitch, int t0, uint32_t dst) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = i * 64 + lane, r = c / CPR, ch = (c % CPR) ^ swz<D>(r);
       const int t = min(t0 + r, tb - 1);
       const long long slot = t < a.sinks ? t : t + shift;
-      const uint32_t dst = l0 + buf * 2 * TB + i * 1024;
-      uint32_t keep;
-      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                   "s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                   : "=&s"(keep) : "v"(kb + slot * a.ks + ch * 16), "v"(vb + slot * a.vs + ch * 16), "s"(dst), "s"(dst + TB) : "memory");
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                   : : "v"(base + slot * pitch + ch * 16), "s"(dst + i * 1024) : "memory", "m0");
     }
+  };
+  auto landed = [] {                                 // all but the NI copies issued last
+    if constexpr (NI == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
   };
   const int gq = lane >> 4, r16 = lane & 15;
   const float c = a.scale * LOG2E;
@@ -115,19 +117,14 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  int t0 = ta + wave * SK, buf = 0;
-  if (t0 < tb) stage(t0, 0);
-  for (; t0 < tb; t0 += 4 * SK, buf ^= 1) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t0 + 4 * SK < tb) {
-      stage(t0 + 4 * SK, buf ^ 1);
-      if constexpr (NI == 8) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    const char* Kt = mine + buf * 2 * TB;
-    const char* Vt = Kt + TB;
+  int t0 = ta + wave * SK;
+  if (t0 < tb) {
+    stage(kb, a.ks, t0, l0);
+    stage(vb, a.vs, t0, l0 + TB);
+  }
+  for (; t0 < tb; t0 += 4 * SK) {
+    const bool more = t0 + 4 * SK < tb;
+    landed();                                        // this tile's keys; its values are on their way
     f32x4 st[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -146,6 +143,8 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
         for (int r = 0; r < 4; ++r)
           if (t0 + u * 16 + 4 * gq + r >= tb) st[u][r] = -INFINITY;
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) stage(kb, a.ks, t0 + 4 * SK, l0);      // the next keys take the place of these
     float mx = m;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -166,6 +165,8 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
         l += e;
         pf[4 * u + r] = (T)e;
       }
+    if (more) landed();                              // this tile's values
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int j = (lane >> 2) & 3, q4 = lane & 3;
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
@@ -180,6 +181,8 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
       o[dt] *= al;
       o[dt] = mfma16<T>(vf, __builtin_bit_cast(s16x8, pf), o[dt]);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) stage(vb, a.vs, t0 + 4 * SK, l0 + TB);
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
