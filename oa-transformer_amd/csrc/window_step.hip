@@ -23,7 +23,7 @@ struct StepArgs {
   char *kc, *vc;
   long long kb, ks, kh, vb, vs, vh;                  // cache strides in bytes: sequence, slot, head
   char* out; long long ldo;
-  float* pieces; int* tickets;
+  float *pieces, *sums; int* tickets;                // [B, Hq, splits, D], [B, Hq, splits, 2] (maximum in base 2, sum), [B, Hkv]
   int B, Hq, Hkv, cap, left, sinks, rolling, splits, turn;
   float scale;
   OatRope rope;
@@ -32,7 +32,12 @@ struct StepArgs {
 // the pieces' sums pass between workgroups of different XCDs: agent-scope accesses go past the L2s that are not shared, so that no
 // fence has to write back and drop whole caches (with __threadfence a workgroup took 100 us instead of 10)
 OAT_DEV void put(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-OAT_DEV float get(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+OAT_DEV void put2(float* p, f32x2 v) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+OAT_DEV f32x2 get2(const float* p) {
+  return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 
 constexpr int SK = 32;                               // keys of a wave's tile
 template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
@@ -43,7 +48,7 @@ template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
 // next keys while it works on these): 64 KB in flight per CU, with 64 KB of LDS a workgroup (D = 128), so that two or more share a CU.  S^T = K Q^T and
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
 // The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
-// new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in the order of the pieces.
+// new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in a fixed order.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -209,9 +214,9 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
     if (parts == 1) {
       reinterpret_cast<T*>(a.out + b * a.ldo)[h * D + d] = (T)(oo / ll);
     } else {
-      float* pc = a.pieces + ((size_t)(b * a.Hq + h) * a.splits + piece) * (D + 2);
-      put(pc + d, oo);
-      if (d == 0) { put(pc + D, mm * c); put(pc + D + 1, ll); }
+      const size_t at = (size_t)(b * a.Hq + h) * a.splits + piece;
+      put(a.pieces + at * D + d, oo);
+      if (d == 0) put2(a.sums + at * 2, f32x2{mm * c, ll});
     }
   }
   if (parts == 1) return;
@@ -223,18 +228,61 @@ __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
   }
   __syncthreads();
   if (!last) return;
-  for (int t = tid; t < G * D; t += 256) {
-    const int h = hk * G + t / D, d = t % D;
-    const float* pc = a.pieces + (size_t)(b * a.Hq + h) * a.splits * (D + 2);
-    float mm = -INFINITY;
-    for (int i = 0; i < parts; ++i) mm = fmaxf(mm, get(pc + i * (D + 2) + D));
-    float ll = 0.f, oo = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const float e = __builtin_amdgcn_exp2f(get(pc + i * (D + 2) + D) - mm);
-      ll += get(pc + i * (D + 2) + D + 1) * e;
-      oo += get(pc + i * (D + 2) + d) * e;
+  // join: the weight of every piece of four heads into the LDS, then each team of D / 2 lanes adds every TEAMS-th piece (eight bytes a
+  // lane, four pieces of four heads in flight), and the teams' sums meet in the LDS
+  constexpr int TEAMS = 512 / D;
+  float* wt = reinterpret_cast<float*>(lds);                           // [4][256]
+  f32x2* red = reinterpret_cast<f32x2*>(lds + 4096);                   // [TEAMS][4][D / 2]
+  const int team = tid / (D / 2), dl = tid % (D / 2);
+  for (int gb = 0; gb < G; gb += 4) {
+    const size_t row0 = (size_t)(b * a.Hq + hk * G + gb) * a.splits;
+    __syncthreads();
+    {
+      // a wave = one head: maximum, sum and weights of its pieces, up to 256
+      f32x2 ml[4];
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = k * 64 + lane;
+        ml[k] = i < parts && gb + wave < G ? get2(a.sums + (row0 + (size_t)wave * a.splits + i) * 2) : f32x2{-INFINITY, 0.f};
+        mm = fmaxf(mm, ml[k][0]);
+      }
+      mm = wave_max(mm);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        ml[k][0] = ml[k][0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[k][0] - mm) : 0.f;
+        ll += ml[k][0] * ml[k][1];
+      }
+      ll = wave_sum(ll);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) wt[wave * 256 + k * 64 + lane] = gb + wave < G ? ml[k][0] / ll : 0.f;
     }
-    reinterpret_cast<T*>(a.out + b * a.ldo)[h * D + d] = (T)(oo / ll);
+    __syncthreads();
+    f32x2 acc[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) acc[g] = f32x2{0.f, 0.f};
+    for (int i = team; i < parts; i += 4 * TEAMS) {
+      f32x2 x[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)                                    // (past the last piece or head: the last one, with weight 0)
+          x[k][g] = get2(a.pieces + (row0 + (size_t)min(g, G - 1 - gb) * a.splits + min(i + k * TEAMS, parts - 1)) * D + 2 * dl);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) acc[g] += (i + k * TEAMS < parts ? wt[g * 256 + i + k * TEAMS] : 0.f) * x[k][g];
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) red[(team * 4 + g) * (D / 2) + dl] = acc[g];
+    __syncthreads();
+    for (int t = tid; t < min(4, G - gb) * (D / 2); t += 256) {
+      f32x2 v = red[t];
+      for (int w = 1; w < TEAMS; ++w) v += red[w * 4 * (D / 2) + t];
+      T* po = reinterpret_cast<T*>(a.out + b * a.ldo) + (hk * G + gb) * D + 2 * t;
+      po[0] = (T)v[0];
+      po[1] = (T)v[1];
+    }
   }
 }
 
@@ -317,12 +365,14 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.cap = cap; a.sinks = sinks; a.rolling = rolling != 0;
   a.left = left < 0 || left > (1 << 29) ? 1 << 29 : left;
   const long long seen = rolling ? cap : min((long long)cap, (long long)sinks + a.left + 1);
-  a.splits = (int)max(1ll, min((long long)most_pieces(B, Hkv), (seen + 255) / 256));
+  // a piece of 512 keys is four tiles a wave; joining two pieces costs about what these take (12 heads, 512 keys: 7.6 us whole, 8.6 us in two)
+  a.splits = (int)max(1ll, min((long long)most_pieces(B, Hkv), (seen + 511) / 512));
   a.turn = rope != nullptr;
   if (rope) a.rope = *rope;
   a.scale = scale;
-  a.tickets = (int*)workspace;
-  a.pieces = (float*)workspace + (size_t)B * Hkv;
+  a.pieces = (float*)workspace;
+  a.sums = a.pieces + (size_t)B * Hq * most_pieces(B, Hkv) * D;
+  a.tickets = (int*)(a.sums + (size_t)B * Hq * most_pieces(B, Hkv) * 2);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(B * Hkv * ((Hq / Hkv + 15) / 16) * a.splits));
 #define STEP_LAUNCH(T, DD)                                                       \
