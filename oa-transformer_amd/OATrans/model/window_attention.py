@@ -33,11 +33,31 @@ def rope_axes(x, pos, rope, heads, head_dim):
     return _RopeFn.apply(x, pos, rope, heads, head_dim)
 
 
-def _parts(qkv, rope, pos, heads, kv_heads, D):
-    """(q, k, v) rows; q and k turned into a new buffer, v where it stands"""
-    n = (heads + kv_heads) * D
-    qk = hip.rope_axes(qkv[:, :n], pos, rope, heads + kv_heads, D) if rope is not None else qkv
-    return qk[:, :heads * D], qk[:, heads * D:n], qkv[:, n:]
+def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse):
+    """-> (out, turned q | k or None): rotary positions into a new buffer (the values stay where they are), attention over it.  The
+    arguments of both calls are columns of two buffers, checked here once, so the calls get addresses."""
+    M, n = qkv.shape[0], (heads + kv_heads) * D
+    what = "window_attention"
+    if qkv.stride(1) != 1 or qkv.dtype not in (torch.bfloat16, torch.float16):
+        raise hip.OatError(f"{what}: qkv must be bf16 or fp16 with unit column stride")
+    if seqs.dtype != torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous() or seqs.device != qkv.device:
+        raise hip.OatError(f"{what}: seqs must be a contiguous int32 [B, 4] on {qkv.device}")
+    lib, dtype, base, ld = hip.lib(), hip._ELEMENTS[qkv.dtype], qkv.data_ptr(), hip._ld(qkv)
+    qk, at, ldqk = None, base, ld
+    if rope is not None:
+        if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[1] != rope.axes or not pos.is_contiguous() or pos.device != qkv.device:
+            raise hip.OatError(f"{what}: pos must be a contiguous int32 [P, {rope.axes}] on {qkv.device}")
+        qk = torch.empty(M, n, dtype=qkv.dtype, device=qkv.device)
+        at, ldqk = qk.data_ptr(), n
+        hip._launch(qkv.device, lib.oat_rope_axes, (base, ld, at, n, dtype, pos.data_ptr(), pos.shape[0], M, heads + kv_heads, D, rope.struct, 0),
+                    "oat_rope_axes")
+    out = (torch.empty if packed else torch.zeros)(M, heads * D, dtype=qkv.dtype, device=qkv.device)
+    size = qkv.element_size()
+    hip._launch(qkv.device, lib.oat_attn_window_fwd, (
+        at, ldqk, at + heads * D * size, ldqk, base + n * size, ld, out.data_ptr(), heads * D, lse.data_ptr() if lse is not None else None,
+        seqs.data_ptr(), seqs.shape[0], longest, longest, M, M, heads, kv_heads, D, dtype, *window, D ** -0.5 if scale is None else scale),
+        "oat_attn_window_fwd")
+    return out, qk
 
 
 class _WindowFn(torch.autograd.Function):
@@ -46,27 +66,25 @@ class _WindowFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed):
-        q, k, v = _parts(qkv, rope, pos, heads, kv_heads, D)
-        make = torch.empty if packed else torch.zeros
-        out = make(qkv.shape[0], heads * D, dtype=qkv.dtype, device=qkv.device)
         lse = torch.empty(qkv.shape[0], heads, dtype=torch.float32, device=qkv.device)
-        hip.attn_window_fwd(q, k, v, seqs, heads, kv_heads, D, longest, longest, *window, scale=scale, out=out, lse=lse)
-        ctx.save_for_backward(q, k, v, out, lse, seqs, pos)
+        out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse)
+        ctx.save_for_backward(qkv, qk, out, lse, seqs, pos)
         ctx.args = heads, kv_heads, D, longest, window, scale, rope, packed
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, seqs, pos = ctx.saved_tensors
+        qkv, qk, out, lse, seqs, pos = ctx.saved_tensors
         heads, kv_heads, D, longest, window, scale, rope, packed = ctx.args
-        n = (heads + kv_heads) * D
-        make = torch.empty if packed else torch.zeros
-        dqkv = make(q.shape[0], n + kv_heads * D, dtype=q.dtype, device=q.device)
-        hip.attn_window_bwd(q, k, v, out, lse, dout.contiguous(), seqs, heads, kv_heads, D, longest, longest, *window, scale=scale,
-                            dq=dqkv[:, :heads * D], dk=dqkv[:, heads * D:n], dv=dqkv[:, n:])
+        n, a = (heads + kv_heads) * D, heads * D
+        qk = qkv if qk is None else qk
+        dqkv = (torch.empty if packed else torch.zeros)(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        hip.attn_window_bwd(qk[:, :a], qk[:, a:n], qkv[:, n:], out, lse, dout.contiguous(), seqs, heads, kv_heads, D, longest, longest, *window,
+                            scale=scale, dq=dqkv[:, :a], dk=dqkv[:, a:n], dv=dqkv[:, n:])
         if rope is not None:
-            hip.rope_axes(dqkv[:, :n], pos, rope, heads + kv_heads, D, out=dqkv[:, :n], inverse=True)
+            turned = dqkv[:, :n]
+            hip.rope_axes(turned, pos, rope, heads + kv_heads, D, out=turned, inverse=True)
         return dqkv, None, None, None, None, None, None, None, None, None, None
 
 
@@ -97,11 +115,10 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
         if right != 0 or (slots < longest and not (left >= 0 and slots == sinks + left + 1)):
             raise hip.OatError("window_attention: a cache belongs to causal attention (right = 0) and needs a slot for every token, or "
                                "sinks + left + 1 slots")
-    q, k, v = _parts(qkv, rope, pos, heads, kv_heads, D)
-    out = (torch.empty if packed else torch.zeros)(qkv.shape[0], heads * D, dtype=qkv.dtype, device=qkv.device)
-    hip.attn_window_fwd(q, k, v, seqs, heads, kv_heads, D, longest, longest, left, right, sinks, scale=scale, out=out)
+    out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, (left, right, sinks), scale, rope, packed, None)
     if cache is not None:
-        hip.window_cache_fill(k, v, seqs, cache[0], cache[1], longest, sinks=sinks)
+        n = (heads + kv_heads) * D
+        hip.window_cache_fill((qkv if qk is None else qk)[:, heads * D:n], qkv[:, n:], seqs, cache[0], cache[1], longest, sinks=sinks)
     return out
 
 

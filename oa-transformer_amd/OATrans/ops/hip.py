@@ -1023,22 +1023,23 @@ def _need(ok, why):
         raise OatError(why)
 
 
-def _launch(device, call, what):
-    """call(stream) on the current stream of `device`, which need not be the current device."""
+def _launch(device, fn, args, what):
+    """fn(*args, stream) on the current stream of `device`, which need not be the current device."""
     if device.type != "cuda":
         raise OatError(f"{what} runs on MI355X only (no CPU path)")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            rc = call(torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
-        rc = call(torch.cuda.current_stream().cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))      # (a Stream object costs more than the call itself)
     if rc != 0:
         _check(rc, what)
 
 
 def _rows(t, columns, dtype, device, what):
     """t is a [rows, >= columns] matrix of dtype with neighbouring columns"""
-    if t.dim() != 2 or t.shape[1] < columns or (t.stride(1) != 1 and t.shape[1] > 1) or t.dtype != dtype or t.device != device:
+    if t.dim() != 2 or t.shape[1] < columns or t.stride(1) != 1 or t.dtype != dtype or t.device != device:
         raise OatError(f"{what}: need [rows, {columns}] of {dtype} on {device} with unit column stride, got {list(t.shape)} {t.dtype} "
                        f"on {t.device}, strides {t.stride()}")
 
@@ -1062,8 +1063,8 @@ def rope_axes(x, pos, rope, heads, head_dim, out=None, inverse=False):
     else:
         _rows(out, heads * head_dim, x.dtype, x.device, "rope_axes: out")
         _need(out.shape[0] == M, "rope_axes: out has another number of rows")
-    _launch(x.device, lambda s: lib().oat_rope_axes(x.data_ptr(), _ld(x), out.data_ptr(), _ld(out), _ELEMENTS[x.dtype], pos.data_ptr(),
-                                                    pos.shape[0], M, heads, head_dim, rope.struct, int(inverse), s), "oat_rope_axes")
+    _launch(x.device, lib().oat_rope_axes, (x.data_ptr(), _ld(x), out.data_ptr(), _ld(out), _ELEMENTS[x.dtype], pos.data_ptr(), pos.shape[0],
+                                            M, heads, head_dim, rope.struct, int(inverse)), "oat_rope_axes")
     return out
 
 
@@ -1108,10 +1109,10 @@ def attn_window_fwd(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, left
     _need(out.shape[0] == q.shape[0], "attn_window_fwd: out has another number of rows than q")
     _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (q.shape[0], heads) and lse.is_contiguous() and lse.device == q.device),
           "attn_window_fwd: lse must be a contiguous fp32 [rows, heads]")
-    _launch(q.device, lambda s: lib().oat_attn_window_fwd(
+    _launch(q.device, lib().oat_attn_window_fwd, (
         q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr() if lse is not None else None,
         seqs.data_ptr(), seqs.shape[0], max_q, max_k, q.shape[0], k.shape[0], heads, kv_heads, head_dim, _ELEMENTS[q.dtype], left, right,
-        sinks, head_dim ** -0.5 if scale is None else scale, s), "oat_attn_window_fwd")
+        sinks, head_dim ** -0.5 if scale is None else scale), "oat_attn_window_fwd")
     return out
 
 
@@ -1137,11 +1138,11 @@ def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, ma
     if workspace is None:
         workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, seqs.shape[0], max_q, max_k, heads, kv_heads, D, left, sinks) // 4, dtype=torch.float32, device=dev)
     _need(workspace.is_contiguous() and workspace.device == dev, what + ": workspace must be contiguous on the same device")
-    _launch(dev, lambda s: lib().oat_attn_window_bwd(
+    _launch(dev, lib().oat_attn_window_bwd, (
         q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr(), dout.data_ptr(), _ld(dout),
         dq.data_ptr(), _ld(dq), dk.data_ptr(), _ld(dk), dv.data_ptr(), _ld(dv), seqs.data_ptr(), seqs.shape[0], max_q, max_k, M, k.shape[0],
         heads, kv_heads, D, _ELEMENTS[dt], left, right, sinks, D ** -0.5 if scale is None else scale, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), s), "oat_attn_window_bwd")
+        workspace.numel() * workspace.element_size()), "oat_attn_window_bwd")
     return dq, dk, dv
 
 
@@ -1181,11 +1182,11 @@ def attn_window_step(qkv, past, k_cache, v_cache, heads, left=-1, sinks=0, rolli
     else:
         _rows(out, heads * D, dt, dev, what + ": out")
         _need(out.shape[0] == B, what + ": one row of out per sequence")
-    _launch(dev, lambda s: lib().oat_attn_window_step(
+    _launch(dev, lib().oat_attn_window_step, (
         qkv.data_ptr(), _ld(qkv), past.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, cap, out.data_ptr(), _ld(out), B, heads,
         kv_heads, D, _ELEMENTS[dt], left, sinks, int(rolling), D ** -0.5 if scale is None else scale,
         rope.struct if rope is not None else None, pos.data_ptr() if rope is not None else None, pieces.data_ptr(),
-        pieces.numel() * pieces.element_size(), s), "oat_attn_window_step")
+        pieces.numel() * pieces.element_size()), "oat_attn_window_step")
     return out
 
 
@@ -1198,6 +1199,6 @@ def window_cache_fill(k, v, seqs, k_cache, v_cache, max_k, sinks=0):
     _rows(v, kv_heads * D, k_cache.dtype, k_cache.device, what + ": v")
     _need(k.shape[0] == v.shape[0], what + ": k and v have different numbers of rows")
     _need(seqs.dtype == torch.int32 and seqs.shape == (B, 4) and seqs.is_contiguous() and seqs.device == k.device, what + ": seqs must be int32 [B, 4]")
-    _launch(k.device, lambda s: lib().oat_window_cache_fill(
+    _launch(k.device, lib().oat_window_cache_fill, (
         k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), seqs.data_ptr(), B, k.shape[0], max_k, k_cache.data_ptr(), v_cache.data_ptr(), strides,
-        cap, kv_heads, D, sinks, s), "oat_window_cache_fill")
+        cap, kv_heads, D, sinks), "oat_window_cache_fill")
