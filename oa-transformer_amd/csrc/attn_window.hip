@@ -459,29 +459,182 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
     }
 }
 
-// the sinks' slabs, added slot by slot: a thread = one key, 8 values of dK or dV
+// The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other through the LDS, and then one adds
+// up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum instead of two (64 instead of 128
+// registers at D = 128), so that two waves fit a SIMD.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
+  constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * ST + 8192];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
+  Place pl;
+  if (!place((a.max_k + 63) / 64, a.Hkv, a.B, pl)) return;
+  const Seq s = load_seq(a, pl.b);
+  const int j0 = pl.tile * 64;
+  if (j0 >= s.nk) return;
+  const int off = s.nk - s.nq;
+  const bool split = a.groups > 0;                                     // the sinks' far queries are the other kernel's (far)
+  auto lo = [&](int j) WIN_INLINE { return j - a.right - off; };       // the queries that see key j
+  auto hi = [&](int j) WIN_INLINE { return !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
+  const int jend = min(j0 + 63, s.nk - 1);
+  const int i0 = max(0, lo(j0)), i1 = !split && j0 < a.sinks ? s.nq - 1 : hi(jend);
+  const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1, count = nt * G;
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
+  const Stager<D> sq(a.ldq), sd(a.lddo);
+  auto stage = [&](int g, int t, int buf) WIN_INLINE {
+    const int i0 = t * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
+    const long long row = s.q0 + i0;
+    const uint32_t l = l0 + buf * ST;
+    sq(a.q + row * a.ldq + h * (D * 2), last, l);
+    sd(a.dout + row * a.lddo + h * (D * 2), last, l + TB);
+    if (wave < 2) {
+      const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                   : : "v"((uint32_t)min(lane, last) * 4u), "s"(src), "s"(l + 2 * TB + wave * 256) : "memory", "m0");
+    }
+  };
+  const int u = wave >> 1;                                             // the wave's half of a tile; 0 adds up dV, 1 dK
+  const int jw = j0 + (wave & 1) * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1), jwe = min(jw + 31, s.nk - 1);
+  const float c = a.scale * LOG2E;
+  s16x8 kf[D / 16], vf[D / 16];
+  load_cols<D>(kf, a.k + (long long)(s.k0 + jc) * a.ldk + pl.h * (D * 2));
+  load_cols<D>(vf, a.v + (long long)(s.k0 + jc) * a.ldv + pl.h * (D * 2));
+  const int ilo = lo(j), ihi = j < s.nk ? hi(j) : -1;
+  const bool sink_w = !split && jwe < a.sinks;                         // the wave's keys are sinks all
+  // queries wlo .. whi see a key of the wave, flo .. fhi see them all
+  const int wlo = lo(jw), whi = !split && jw < a.sinks ? s.nq - 1 : hi(jwe);
+  const int flo = lo(jwe), fhi = sink_w ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);
+  f32x16 sum[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[dt][r] = 0.f;
+  char* const mine = lds + 2 * ST + wave * 2048 + lane * 16;
+  const char* const other = lds + 2 * ST + (wave ^ 2) * 2048 + lane * 16;
+  int g1 = 0, t1 = t0;                                                 // head and tile that is staged next
+  if (count) {
+    stage(0, t0, 0);
+    t1 = t0 + 1;
+  }
+  int t = t0;
+  for (int n = 0; n < count; ++n) {
+    tile_barrier();
+    if (t1 == t0 + nt) { t1 = t0; ++g1; }
+    if (n + 1 < count) stage(g1, t1, (n + 1) & 1);
+    const int iu = t * TILE + u * 32;
+    const char* Qt = lds + (n & 1) * ST;
+    const char* Dt = Qt + TB;
+    const float* Lt = reinterpret_cast<const float*>(Dt + TB) + u * 32 + 4 * half;
+    s16x8 keep[2];
+    if (jw >= s.nk || iu > whi || iu + 31 < wlo) {
+      keep[0] = keep[1] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      *reinterpret_cast<s16x8*>(mine) = keep[0];
+      *reinterpret_cast<s16x8*>(mine + 1024) = keep[0];
+    } else {
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
+        dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(Lt + 8 * g), de = *reinterpret_cast<const f32x4*>(Lt + 64 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -ls[e]));
+          dp[r] -= de[e];
+        }
+      }
+      if (iu < flo || iu + 31 > fhi) {
+        const Bounds bd{ilo - iu - 4 * half, ihi - iu - 4 * half, 0};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] *= st[r];
+      const s16x8 p0 = pack8<T>(st, 0), p1 = pack8<T>(st, 1), s0 = pack8<T>(dp, 0), s1 = pack8<T>(dp, 1);
+      *reinterpret_cast<s16x8*>(mine) = u ? p0 : s0;
+      *reinterpret_cast<s16x8*>(mine + 1024) = u ? p1 : s1;
+      keep[0] = u ? s0 : p0;
+      keep[1] = u ? s1 : p1;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    s16x8 got[2];
+    got[0] = *reinterpret_cast<const s16x8*>(other);
+    got[1] = *reinterpret_cast<const s16x8*>(other + 1024);
+    const char* Xt = u ? Qt : Dt;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        sum[dt] = mfma32<T>(col_frag32<D>(Xt, u * 32 + h * 16, dt), keep[h], sum[dt]);
+        sum[dt] = mfma32<T>(col_frag32<D>(Xt, (1 - u) * 32 + h * 16, dt), got[h], sum[dt]);
+      }
+    if (++t == t0 + nt) t = t0;
+    ++t1;
+  }
+  if (split && jw < a.sinks) {
+    // the window's own slot of the slabs
+    const int slots = 2 * a.pieces + 1;
+    float* sl = a.slabs + (((size_t)(pl.b * a.Hkv + pl.h) * a.groups + jw / 32) * slots + slots - 1) * (2 * D * 32) + (u ? 0 : D * 32) + (lane & 31);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sl[(dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3)) * 32] = sum[dt][r];
+    return;
+  }
+  if (j >= s.nk) return;
+  const float f = u ? a.scale : 1.f;
+  char* po = (u ? a.dk + (long long)(s.k0 + j) * a.lddk : a.dv + (long long)(s.k0 + j) * a.lddv) + pl.h * (D * 2);
+  typedef __attribute__((ext_vector_type(4))) T T4;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      T4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (T)(sum[dt][4 * g + e] * f);
+      *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = x;
+    }
+}
+
+// the sinks' slabs, added slot by slot (every eighth one a thread, then the eight): a workgroup = 32 keys, 8 values of dK or dV each
 template <class T, int D>
 __global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
-  const int key = threadIdx.x & 31, d8 = blockIdx.y * 8 + (threadIdx.x >> 5);          // d8: 0 .. 2 D / 8
+  __shared__ float part[8][8][32];
+  const int key = threadIdx.x & 31, w = threadIdx.x >> 5, d8 = blockIdx.y;              // d8: 0 .. 2 D / 8
   const int group = blockIdx.x % a.groups, h = blockIdx.x / a.groups % a.Hkv, b = blockIdx.x / a.groups / a.Hkv;
   const Seq s = load_seq(a, b);
-  const int j = group * 32 + key;
-  if (group * 32 >= a.sinks || j >= s.nk) return;
+  if (group * 32 >= min(a.sinks, s.nk)) return;
   const int slots = 2 * a.pieces + 1;
-  const float* sl = a.slabs + ((size_t)blockIdx.x * slots) * (2 * D * 32) + d8 * 8 * 32 + key;
+  const float* sl = a.slabs + ((size_t)blockIdx.x * slots + w) * (2 * D * 32) + d8 * 8 * 32 + key;
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < slots; ++i, sl += 2 * D * 32) {
+  for (int i = w; i < slots; i += 8, sl += 8 * 2 * D * 32) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] += sl[e * 32];
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[w][e][key] = x[e];
+  __syncthreads();
+  const int j = group * 32 + key;
+  if (w || j >= s.nk) return;
   const bool is_v = d8 >= D / 8;
   typedef __attribute__((ext_vector_type(8))) T T8;
   T8 y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = (T)(is_v ? x[e] : x[e] * a.scale);
+  for (int e = 0; e < 8; ++e) {
+    float v = part[0][e][key];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += part[k][e][key];
+    y[e] = (T)(is_v ? v : v * a.scale);
+  }
   char* p = is_v ? a.dv + (long long)(s.k0 + j) * a.lddv : a.dk + (long long)(s.k0 + j) * a.lddk;
   *reinterpret_cast<T8*>(p + h * (D * 2) + (is_v ? d8 - D / 8 : d8) * 16) = y;
 }
@@ -489,11 +642,12 @@ __global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
 // how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries; 0 groups: the sinks' own tiles walk all
 // queries.  That takes max_q / 64 steps where a window's tile takes (left + right + 128) / 64: split where it is over 512 queries longer.
 struct FarSplit { int groups, pieces; };
-static FarSplit far_split(int B, int Hq, int Hkv, int max_q, int max_k, int left, int sinks) {
+static FarSplit far_split(int B, int Hq, int Hkv, int D, int max_q, int max_k, int left, int sinks) {
   const long long rows = min((long long)max_q, (long long)max_k - left);
   if (sinks < 1 || rows <= 512 || B < 1) return {0, 0};
   const int groups = (min(sinks, max_k) + 31) / 32;
-  const long long want = 512 / max(1ll, (long long)B * Hkv * groups);
+  // as many workgroups as stay resident: two a CU with heads of 64, one with heads of 128
+  const long long want = (D == 64 ? 512 : 256) / max(1ll, (long long)B * Hkv * groups);
   return {groups, (int)max(1ll, min(want, rows * (Hq / Hkv) / 256))};
 }
 static size_t slab_floats(const FarSplit& f, int B, int Hkv, int D) {
@@ -514,7 +668,7 @@ static int window_wrong(const char* what, const void* seqs, int B, int max_q, in
   else if ((uintptr_t)seqs % 16) w = "the table of sequences is not aligned to 16 bytes";
   else if (sinks < 0 || sinks > (1 << 29)) w = "sinks of 0 to 2^29";
   else if (!(scale > 0.f && scale < 1e30f)) w = "the scale is not a positive number";
-  else if ((long long)B * Hq * (max_q / 128 + 1) >= (1ll << 30) || (long long)B * Hkv * (max_k / 128 + 1) >= (1ll << 30)) w = "more than 2^30 tiles";
+  else if ((long long)B * Hq * (max_q / 128 + 1) >= (1ll << 30) || (long long)B * Hkv * (max_k / 64 + 1) >= (1ll << 30)) w = "more than 2^30 tiles";
   if (!w) return 0;
   char msg[160];
   snprintf(msg, sizeof msg, "%s: %s", what, w);
@@ -531,7 +685,13 @@ using namespace oat;
 #define WIN_Q(T, D) win_bwd_q_kernel<T, D>
 #define WIN_FAR(T, D) win_bwd_kv_kernel<T, D, true>
 #define WIN_KV(T, D) win_bwd_kv_kernel<T, D, false>
+#define WIN_KV2(T, D) win_bwd_kv2_kernel<T, D>
 #define WIN_SINK(T, D) win_bwd_sink_kernel<T, D>
+#define WIN_LAUNCH1(kernel, DD, grid)                                                                                \
+  do {                                                                                                               \
+    if (dtype == 0) OAT_LAUNCH((kernel(bf16, DD)), dim3(grid), dim3(256), 0, s, a);                                  \
+    else OAT_LAUNCH((kernel(_Float16, DD)), dim3(grid), dim3(256), 0, s, a);                                         \
+  } while (0)
 #define WIN_LAUNCH(kernel, blocks) WIN_LAUNCH2(kernel, dim3(place_grid(blocks)))
 #define WIN_LAUNCH2(kernel, grid)                                                                                    \
   do {                                                                                                               \
@@ -564,7 +724,7 @@ extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, 
 
 extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max_q, int max_k, int Hq, int Hkv, int D, int left, int sinks) {
   if (rows_q < 0 || Hq < 1 || Hkv < 1 || D < 1) return 0;
-  return ((size_t)rows_q * Hq * 2 + slab_floats(far_split(B, Hq, Hkv, max_q, max_k, far(left), sinks), B, Hkv, D)) * 4;
+  return ((size_t)rows_q * Hq * 2 + slab_floats(far_split(B, Hq, Hkv, D, max_q, max_k, far(left), sinks), B, Hkv, D)) * 4;
 }
 
 extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
@@ -593,12 +753,17 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
   if (max_q && rows_q) WIN_LAUNCH(WIN_Q, (long long)B * Hq * ((max_q + 127) / 128));
-  const FarSplit f = rows_q ? far_split(B, Hq, Hkv, max_q, max_k, a.left, sinks) : FarSplit{0, 0};
+  const FarSplit f = rows_q ? far_split(B, Hq, Hkv, D, max_q, max_k, a.left, sinks) : FarSplit{0, 0};
   a.groups = f.groups;
   a.pieces = f.pieces;
   a.slabs = a.delta + (size_t)rows_q * Hq;
   if (max_k && rows_k && f.groups) WIN_LAUNCH(WIN_FAR, (long long)B * Hkv * f.groups * f.pieces);
-  if (max_k && rows_k) WIN_LAUNCH(WIN_KV, (long long)B * Hkv * ((max_k + 127) / 128));
-  if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 64));
+  if (max_k && rows_k) {
+    // heads of 64: both sums of 32 keys fit a wave beside another wave's (two 16-frame clips 180 us, shared in pairs 194); heads of 128:
+    // they do not (six packed texts 182 us, in pairs 138)
+    if (D == 64) WIN_LAUNCH1(WIN_KV, 64, place_grid((long long)B * Hkv * ((max_k + 127) / 128)));
+    else WIN_LAUNCH1(WIN_KV2, 128, place_grid((long long)B * Hkv * ((max_k + 63) / 64)));
+  }
+  if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 8));
   return check_launch("attn_window_bwd");
 }
