@@ -562,18 +562,17 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
       keep[0] = u ? s0 : p0;
       keep[1] = u ? s1 : p1;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    s16x8 got[2];
-    got[0] = *reinterpret_cast<const s16x8*>(other);
-    got[1] = *reinterpret_cast<const s16x8*>(other + 1024);
     const char* Xt = u ? Qt : Dt;
+    auto add = [&](const s16x8 (&x)[2], int half_of_tile) WIN_INLINE {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        sum[dt] = mfma32<T>(col_frag32<D>(Xt, u * 32 + h * 16, dt), keep[h], sum[dt]);
-        sum[dt] = mfma32<T>(col_frag32<D>(Xt, (1 - u) * 32 + h * 16, dt), got[h], sum[dt]);
-      }
+        for (int dt = 0; dt < D / 32; ++dt) sum[dt] = mfma32<T>(col_frag32<D>(Xt, half_of_tile * 32 + h * 16, dt), x[h], sum[dt]);
+    };
+    add(keep, u);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const s16x8 got[2] = {*reinterpret_cast<const s16x8*>(other), *reinterpret_cast<const s16x8*>(other + 1024)};
+    add(got, 1 - u);
     if (++t == t0 + nt) t = t0;
     ++t1;
   }
