@@ -123,6 +123,7 @@ struct WinArgs {
   const int4* seqs;                     // first query row, queries, first key row, keys
   float* slabs;                         // backward: the sinks' sums (win_bwd_kv_kernel)
   int B, Hq, Hkv, left, right, sinks, max_q, max_k, rows_q, rows_k;
+  int run;                              // tiles that go to one XCD together
   int groups, pieces;                   // how the sinks' far queries are split
   float scale;
 };
@@ -134,19 +135,30 @@ OAT_DEV Seq load_seq(const WinArgs& a, int b) {
                   (long long)s.z + s.w <= a.rows_k;
   return ok ? Seq{s.x, s.y, s.z, s.w} : Seq{0, 0, 0, 0};
 }
-// blockIdx -> (tile, head, sequence).  Workgroups go to the 8 XCDs in turn: each XCD gets a contiguous share of the (sequence, head,
-// tile) list, so the tiles of one head and the heads that share keys meet in one L2.
+// blockIdx -> (tile, head, sequence).  Workgroups go to the 8 XCDs in turn; the (sequence, head, tile) list is dealt to the XCDs in runs of
+// a.run tiles, which share keys in one L2 (deal_run below).
 struct Place { int b, h, tile; };
-OAT_DEV bool place(int tiles, int heads, int B, Place& p) {
-  const int per = gridDim.x >> 3;
-  const int i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (i >= tiles * heads * B) return false;
-  p.tile = i % tiles;
-  p.h = i / tiles % heads;
-  p.b = i / tiles / heads;
+OAT_DEV bool place(const WinArgs& a, int tiles, int heads, Place& p) {
+  const int k = blockIdx.x >> 3, c = k / a.run, i = (c * 8 + (blockIdx.x & 7)) * a.run + k - c * a.run;
+  if (i >= tiles * heads * a.B) return false;
+  const int bh = i / tiles;
+  p.tile = i - bh * tiles;
+  p.b = bh / heads;
+  p.h = bh - p.b * heads;
   return true;
 }
-inline unsigned place_grid(long long n) { return (unsigned)((n + 7) / 8 * 8); }
+// The length of a run.  Whole key heads (with the query heads that share them) where they come out even; in a batch of different lengths
+// single heads, so that every XCD gets some of each sequence (six packed texts: forward 83 us with one contiguous share an XCD, 64 us
+// so); with few heads an eighth of the list, or - different lengths again - small runs.
+inline int deal_run(int B, int heads, int group, int tiles, long long rows, int longest) {
+  const long long units = (long long)B * heads, n = units * tiles;
+  const bool ragged = rows * 10 < 9ll * B * longest;
+  auto even = [](long long u) { return u % 8 == 0 || u >= 64; };
+  if (!ragged && even(units / group)) return tiles * group;
+  if (even(units)) return tiles;
+  return (int)(ragged ? (n / 64) | 1 : (n + 7) / 8);
+}
+inline unsigned deal_grid(long long n, int run) { return (unsigned)((n + 8ll * run - 1) / (8ll * run) * (8ll * run)); }
 
 // The visibility of the pair that register r of a C fragment holds, with the fixed side (a query's keys lo .. hi and sinks, or a key's
 // queries) folded into bounds on the register's row number: row <= hi and (row >= lo or row < sink), no branches.

@@ -14,7 +14,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TB];         // K x 2, V x 2
   const int tiles = (a.max_q + 127) / 128;
   Place pl;
-  if (!place(tiles, a.Hq, a.B, pl)) return;
+  if (!place(a, tiles, a.Hq, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int i0 = (tiles - 1 - pl.tile) * 128;                          // causal rows are longest at the end: those first
   if (i0 >= s.nq) return;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
   const int tiles = (a.max_q + 127) / 128;
   Place pl;
-  if (!place(tiles, a.Hq, a.B, pl)) return;
+  if (!place(a, tiles, a.Hq, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int i0 = (tiles - 1 - pl.tile) * 128;
   if (i0 >= s.nq) return;
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
     pl.h = i / a.pieces / a.groups % a.Hkv;
     pl.b = i / a.pieces / a.groups / a.Hkv;
   } else {
-    if (!place((a.max_k + 127) / 128, a.Hkv, a.B, pl)) return;
+    if (!place(a, (a.max_k + 127) / 128, a.Hkv, pl)) return;
   }
   const Seq s = load_seq(a, pl.b);
   const int j0 = far ? group * 32 : pl.tile * 128;
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * ST + 8192];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
   Place pl;
-  if (!place((a.max_k + 63) / 64, a.Hkv, a.B, pl)) return;
+  if (!place(a, (a.max_k + 63) / 64, a.Hkv, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int j0 = pl.tile * 64;
   if (j0 >= s.nk) return;
@@ -691,7 +691,7 @@ using namespace oat;
     if (dtype == 0) OAT_LAUNCH((kernel(bf16, DD)), dim3(grid), dim3(256), 0, s, a);                                  \
     else OAT_LAUNCH((kernel(_Float16, DD)), dim3(grid), dim3(256), 0, s, a);                                         \
   } while (0)
-#define WIN_LAUNCH(kernel, blocks) WIN_LAUNCH2(kernel, dim3(place_grid(blocks)))
+#define WIN_LAUNCH(kernel, grid) WIN_LAUNCH2(kernel, dim3(grid))
 #define WIN_LAUNCH2(kernel, grid)                                                                                    \
   do {                                                                                                               \
     const dim3 g_ = (grid);                                                                                          \
@@ -717,7 +717,9 @@ extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  WIN_LAUNCH(WIN_FWD, (long long)B * Hq * ((max_q + 127) / 128));
+  const int tiles = (max_q + 127) / 128;
+  a.run = deal_run(B, Hq, Hq / Hkv, tiles, rows_q, max_q);
+  WIN_LAUNCH(WIN_FWD, deal_grid((long long)B * Hq * tiles, a.run));
   return check_launch("attn_window_fwd");
 }
 
@@ -751,7 +753,11 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  if (max_q && rows_q) WIN_LAUNCH(WIN_Q, (long long)B * Hq * ((max_q + 127) / 128));
+  if (max_q && rows_q) {
+    const int tiles = (max_q + 127) / 128;
+    a.run = deal_run(B, Hq, Hq / Hkv, tiles, rows_q, max_q);
+    WIN_LAUNCH(WIN_Q, deal_grid((long long)B * Hq * tiles, a.run));
+  }
   const FarSplit f = rows_q ? far_split(B, Hq, Hkv, D, max_q, max_k, a.left, sinks) : FarSplit{0, 0};
   a.groups = f.groups;
   a.pieces = f.pieces;
@@ -760,8 +766,11 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   if (max_k && rows_k) {
     // heads of 64: both sums of 32 keys fit a wave beside another wave's (two 16-frame clips 180 us, shared in pairs 194); heads of 128:
     // they do not (six packed texts 182 us, in pairs 138)
-    if (D == 64) WIN_LAUNCH1(WIN_KV, 64, place_grid((long long)B * Hkv * ((max_k + 127) / 128)));
-    else WIN_LAUNCH1(WIN_KV2, 128, place_grid((long long)B * Hkv * ((max_k + 63) / 64)));
+    const int tiles = D == 64 ? (max_k + 127) / 128 : (max_k + 63) / 64;
+    a.run = deal_run(B, Hkv, 1, tiles, rows_k, max_k);
+    const unsigned grid = deal_grid((long long)B * Hkv * tiles, a.run);
+    if (D == 64) WIN_LAUNCH1(WIN_KV, 64, grid);
+    else WIN_LAUNCH1(WIN_KV2, 128, grid);
   }
   if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 8));
   return check_launch("attn_window_bwd");
