@@ -147,16 +147,16 @@ OAT_DEV bool place(const WinArgs& a, int tiles, int heads, Place& p) {
   p.h = bh - p.b * heads;
   return true;
 }
-// The length of a run.  Whole key heads (with the query heads that share them) where they come out even; in a batch of different lengths
-// single heads, so that every XCD gets some of each sequence (six packed texts: forward 83 us with one contiguous share an XCD, 64 us
-// so); with few heads an eighth of the list, or - different lengths again - small runs.
+// The length of a run.  In a batch of different lengths short runs of an odd length, so that every XCD gets some of each sequence and of
+// its empty places (six packed texts, from one contiguous share an XCD: forward 83 -> 65 us, dQ 105 -> 84, dK and dV 137 -> 107; whole
+// heads: 64, 82, 130).  Else whole key heads with the query heads that share them, or single heads, where they come out even, or an
+// eighth of the list.
 inline int deal_run(int B, int heads, int group, int tiles, long long rows, int longest) {
-  const long long units = (long long)B * heads, n = units * tiles;
-  const bool ragged = rows * 10 < 9ll * B * longest;
+  const long long units = (long long)B * heads;
+  if (rows * 10 < 9ll * B * longest) return 5;
   auto even = [](long long u) { return u % 8 == 0 || u >= 64; };
-  if (!ragged && even(units / group)) return tiles * group;
-  if (even(units)) return tiles;
-  return (int)(ragged ? (n / 64) | 1 : (n + 7) / 8);
+  if (even(units / group)) return tiles * group;
+  return even(units) ? tiles : (int)((units * tiles + 7) / 8);
 }
 inline unsigned deal_grid(long long n, int run) { return (unsigned)((n + 8ll * run - 1) / (8ll * run) * (8ll * run)); }
 
