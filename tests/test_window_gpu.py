@@ -92,6 +92,19 @@ def test_rope_axes_unaligned_rows_and_gradient():
     within(g, ref, 2.0 ** -20 * w.double().abs().max().item() * torch.ones_like(ref), "gradient")
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_rope_axes_large_output(inter):
+    """Over 96 MB of output the stores bypass the caches: the same values, to the last row."""
+    hip = _hip()
+    rope = hip.RopeAxes((48,), interleaved=inter)                                   # 16 of 64 values pass through
+    M, heads = 35000, 24
+    x = torch.randn(M, heads * 64, dtype=BF, device=DEV, generator=torch.Generator(DEV).manual_seed(3))
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    out = hip.rope_axes(x, pos, rope, heads, 64)
+    for a, b in ((0, 10000), (10000, 20000), (20000, 30000), (30000, M)):
+        assert torch.equal(out[a:b], hip.rope_axes(x[a:b], pos[a:b], rope, heads, 64))
+
+
 # ---------------------------------------------------------------------------------------------- attention
 # queries, keys, Hq, Hkv, D, left, right, sinks
 ATTN = [
