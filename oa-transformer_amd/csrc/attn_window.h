@@ -102,11 +102,11 @@ OAT_DEV float both_halves(float v, bool max) {
   const float x = __builtin_bit_cast(float, (int)r[0]), y = __builtin_bit_cast(float, (int)r[1]);
   return max ? fmaxf(x, y) : x + y;
 }
-// every wave's copies have landed and every wave is done reading what the next copies overwrite.  The wait is the builtin (vmcnt 0,
-// lgkmcnt 0), not asm: the compiler then knows that its own earlier loads are done and puts no wait for them into the loop, which
-// would wait for the next tile's copies too.
+// every wave's copies have landed and every wave is done reading what the next copies overwrite.  The compiler does not know of the
+// copies, so the wait for them is asm; the builtin (vmcnt 0, lgkmcnt 0) after it tells the compiler that its own earlier loads are done:
+// it would put waits for these into the loop, and those would wait for the next tile's copies too.
 OAT_DEV void tile_barrier() {
-  asm volatile("" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x70);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");

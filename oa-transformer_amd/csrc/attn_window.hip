@@ -640,10 +640,11 @@ __global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
 
 // how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries; 0 groups: the sinks' own tiles walk all
 // queries.  That takes max_q / 64 steps where a window's tile takes (left + right + 128) / 64: split where it is over 512 queries longer.
+// (Of many sinks - over 512 keys - the tiles themselves are enough workgroups, and the slabs would be large.)
 struct FarSplit { int groups, pieces; };
 static FarSplit far_split(int B, int Hq, int Hkv, int D, int max_q, int max_k, int left, int sinks) {
   const long long rows = min((long long)max_q, (long long)max_k - left);
-  if (sinks < 1 || rows <= 512 || B < 1) return {0, 0};
+  if (sinks < 1 || min(sinks, max_k) > 512 || rows <= 512 || B < 1) return {0, 0};
   const int groups = (min(sinks, max_k) + 31) / 32;
   // as many workgroups as stay resident: two a CU with heads of 64, one with heads of 128
   const long long want = (D == 64 ? 512 : 256) / max(1ll, (long long)B * Hkv * groups);
@@ -667,7 +668,7 @@ static int window_wrong(const char* what, const void* seqs, int B, int max_q, in
   else if ((uintptr_t)seqs % 16) w = "the table of sequences is not aligned to 16 bytes";
   else if (sinks < 0 || sinks > (1 << 29)) w = "sinks of 0 to 2^29";
   else if (!(scale > 0.f && scale < 1e30f)) w = "the scale is not a positive number";
-  else if ((long long)B * Hq * (max_q / 128 + 1) >= (1ll << 30) || (long long)B * Hkv * (max_k / 64 + 1) >= (1ll << 30)) w = "more than 2^30 tiles";
+  else if ((long long)B * Hq * (max_q / 128 + 1) >= (1ll << 22) || (long long)B * Hkv * (max_k / 64 + 1) >= (1ll << 22)) w = "more than 2^22 tiles";
   if (!w) return 0;
   char msg[160];
   snprintf(msg, sizeof msg, "%s: %s", what, w);

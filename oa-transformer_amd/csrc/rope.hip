@@ -107,9 +107,11 @@ static int rope_run(const void* x, long long ldx, void* out, long long ldo, cons
   const int np = rope->n_pairs;
   // about one angle per thread, but no fewer workgroups than four per CU while rows last
   a.rows = max(1, min(256 / np, M / 1024));
+  if (M / a.rows >= 1 << 22) a.rows = 1024 / np;                       // (a launch holds 2^32 threads)
   const bool vec = (rope->interleaved ? (2 * np) % N : np % N) == 0 && (dim - 2 * np) % N == 0 && dim % N == 0 && ldx % N == 0 && ldo % N == 0 &&
                    ((uintptr_t)x | (uintptr_t)out) % 16 == 0;
-  const int blocks = (M + a.rows - 1) / a.rows;
+  const int blocks = (int)(((long long)M + a.rows - 1) / a.rows);
+  if (blocks >= 1 << 23) { set_error("rope_axes: more rows than a launch can hold (2^23 workgroups)"); return -2; }
   const bool far = (long long)M * heads * dim * (long long)sizeof(T) > FAR_BYTES;
   if (vec && far) OAT_LAUNCH((rope_kernel<T, true, true>), dim3(blocks), dim3(256), 0, s, a);
   else if (vec) OAT_LAUNCH((rope_kernel<T, true, false>), dim3(blocks), dim3(256), 0, s, a);

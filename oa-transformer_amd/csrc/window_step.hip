@@ -341,11 +341,11 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
                                     void* out, long long ldo, int B, int Hq, int Hkv, int D, int dtype, int left, int sinks, int rolling,
                                     float scale, const OatRope* rope, const int* pos, void* workspace, size_t workspace_bytes, void* stream) {
   const char* me = "attn_window_step";
+  if (B == 0) return 0;
   if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
   if (dtype != 0 && dtype != 1) return fail(me, "element type: 0 (bf16) or 1 (fp16)");
   if (Hq < 1 || Hq % Hkv) return fail(me, "the query heads are not a multiple of the key heads");
   if (!(scale > 0.f && scale < 1e30f)) return fail(me, "the scale is not a positive number");
-  if (B == 0) return 0;
   if (!qkv || !out || !past) return fail(me, "qkv, out and the counts of past tokens are needed");
   if (((uintptr_t)qkv | (uintptr_t)out) % 16 || ldqkv % 8 || ldo % 8 || ldqkv < (long long)(Hq + 2 * Hkv) * D || ldo < (long long)Hq * D)
     return fail(me, "qkv and out need 16-byte aligned rows of all their heads");
@@ -356,7 +356,7 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
   }
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < oat_attn_window_step_workspace_bytes(B, Hq, Hkv, D))
     return fail(me, "the workspace is too small, or not aligned to 16 bytes");
-  if ((long long)B * Hkv * ((Hq / Hkv + 15) / 16) * most_pieces(B, Hkv) >= (1ll << 31)) return fail(me, "more than 2^31 pieces");
+  if ((long long)B * Hkv * ((Hq / Hkv + 15) / 16) * most_pieces(B, Hkv) >= (1ll << 23)) return fail(me, "more than 2^23 pieces");
   StepArgs a{};
   a.qkv = (const char*)qkv; a.ldqkv = ldqkv * 2; a.past = past; a.pos = pos;
   a.kc = (char*)kc; a.vc = (char*)vc;
@@ -392,9 +392,10 @@ extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v
                                      int max_k, void* kc, void* vc, const long long* strides, int cap, int Hkv, int D, int sinks,
                                      void* stream) {
   const char* me = "window_cache_fill";
+  if (B == 0) return 0;
   if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
   if (rows_k < 0 || max_k < 0 || B > 65535) return fail(me, "no rows, or more than 65535 sequences");
-  if (B == 0 || rows_k == 0 || max_k == 0) return 0;
+  if (rows_k == 0 || max_k == 0) return 0;
   if (!k || !v || !seqs || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)seqs) % 16 || ldk % 8 || ldv % 8 || ldk < (long long)Hkv * D || ldv < (long long)Hkv * D)
     return fail(me, "k, v need 16-byte aligned rows of all key heads, and the table of sequences 16 bytes");
   FillArgs a{};

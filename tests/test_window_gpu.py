@@ -127,6 +127,9 @@ ATTN = [
     ([1500, 1], None, 2, 1, 128, 50, 50, 1),
     ([1300, 700], None, 4, 1, 128, 100, 0, 40),                                       # the sinks' far queries are split over workgroups
     ([900, 20], [1400, 900], 4, 2, 64, 60, 10, 3),
+    ([1500], None, 1, 1, 64, 100, 0, 600),                                            # many sinks: their own tiles walk all queries
+    ([40] * 9 + [0, 300], None, 3, 3, 64, 20, 5, 2),                                  # a ragged batch: places of the list that are empty
+    ([130] * 5, None, 8, 2, 128, -1, 0, 0),                                           # an even one, dealt by key heads
 ]
 
 
@@ -383,6 +386,37 @@ def test_attn_window_step_far_slots():
     ref = hip.attn_window_step(qkv, torch.tensor([303], dtype=torch.int32, device=DEV), ks, vs, 8, left=299, sinks=4)
     u = half_step(BF)
     within(out, ref.double(), 4 * u * ref.double().abs() + 4 * u * vs.double().abs().max().item(), "far")
+
+
+def test_empty_batches_are_no_work():
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    none = hip.seq_table([])
+    q = rnd(5, 192)
+    out = wa.window_attention(q, none, 1, 1, 64, longest=0)
+    assert (out == 0).all() and out.shape == (5, 64)
+    empty = rnd(0, 192)
+    assert wa.window_attention(empty, none, 1, 1, 64, longest=0).shape == (0, 64)
+    assert wa.window_attention(empty, hip.seq_table([0, 0]), 1, 1, 64, longest=0).shape == (0, 64)
+    caches = torch.zeros(0, 9, 1, 64, dtype=BF, device=DEV)
+    past = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert hip.attn_window_step(empty, past, caches, caches.clone(), 1).shape == (0, 64)
+    hip.window_cache_fill(rnd(0, 64), rnd(0, 64), none, caches, caches.clone(), 0)
+    rope = hip.RopeAxes((64,))
+    assert hip.rope_axes(rnd(0, 64), torch.zeros(1, 1, dtype=torch.int32, device=DEV), rope, 1, 64).shape == (0, 64)
+
+
+def test_step_pieces_are_read_fresh():
+    """The pieces' sums pass between workgroups through memory that earlier calls used: every one of many calls with other data gives
+    what a new workspace gives."""
+    hip = _hip()
+    B, cap, Hq, Hkv, D = 2, 6000, 8, 2, 128
+    kc, vc = rnd(B, cap, Hkv, D, seed=1), rnd(B, cap, Hkv, D, seed=2)
+    pieces = hip.window_step_workspace(B, Hq, Hkv, D)
+    for k in range(12):
+        past = torch.tensor([5999 - 311 * k, 400 * k], dtype=torch.int32, device=DEV)
+        x = rnd(B, (Hq + 2 * Hkv) * D, seed=50 + k)
+        assert torch.equal(hip.attn_window_step(x, past, kc, vc, Hq, pieces=pieces), hip.attn_window_step(x, past, kc, vc, Hq)), k
 
 
 @pytest.mark.parametrize("cap,sinks,lens", [(40, 0, [40, 1]), (20, 4, [19, 20, 21, 100]), (16, 15, [3, 200]), (5, 9, [4, 5])])
