@@ -170,19 +170,29 @@ struct Bounds {
   }
 };
 // masks the scores of 32 keys (the first at jb for this lane's half; lo .. hi and the sinks are what its query sees).  Most tiles that
-// are not seen whole lie across one edge only: one comparison each.
-template <bool ZERO> OAT_DEV void mask_keys(f32x16& S, int jb, int lo, int hi, int sinks, bool edge_lo, bool edge_hi) {
-  const float no = ZERO ? 0.f : -INFINITY;
+// are not seen whole lie across one edge only: one comparison each.  (The empty asm keeps the comparisons behind the caller's branch.)
+OAT_DEV void mask_keys(f32x16& S, int jb, int lo, int hi, int sinks, bool edge_lo, bool edge_hi) {
+  asm volatile("" : "+v"(jb));
   const Bounds bd{lo - jb, hi - jb, sinks - jb};
   if (!edge_lo) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) <= bd.hi ? S[r] : no;
-  } else if (!edge_hi && sinks <= jb) {
+    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) <= bd.hi ? S[r] : -INFINITY;
+  } else if (!edge_hi && sinks <= __builtin_amdgcn_readfirstlane(jb)) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) >= bd.lo ? S[r] : no;
+    for (int r = 0; r < 16; ++r) S[r] = 8 * (r >> 2) + (r & 3) >= bd.lo ? S[r] : -INFINITY;
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) S[r] = bd.sees(r) ? S[r] : no;
+    for (int r = 0; r < 16; ++r) S[r] = bd.sees(r) ? S[r] : -INFINITY;
+  }
+}
+// and of 32 queries, ilo .. ihi being those that see this lane's key
+OAT_DEV void mask_queries(f32x16& S, int ib, int ilo, int ihi) {
+  asm volatile("" : "+v"(ib));
+  const int lo = ilo - ib, hi = ihi - ib;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r >> 2) + (r & 3);
+    S[r] = (row >= lo) & (row <= hi) ? S[r] : -INFINITY;
   }
 }
 // the key tiles (of 64) that queries at positions p0 .. p1 see: those of the sinks, then those of the window

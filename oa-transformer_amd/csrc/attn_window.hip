@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
       for (int dt = 0; dt < D / 32; ++dt) vf[h][dt] = col_frag32<D>(V, (1 - u) * 32 + h * 16, dt);
     const int j0 = kt.at(n) * TILE + u * 32;
     const bool edge_hi = j0 + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = j0 < wp1 - a.left && j0 + 31 >= a.sinks;
-    if (edge_lo | edge_hi) mask_keys<false>(S, j0 + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
+    if (edge_lo | edge_hi) mask_keys(S, j0 + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
     if (!all_begun) {
       const float mx = row_max(S);
       if (!begun && mx > -INFINITY) {
@@ -220,10 +220,10 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   const char* vb = a.v + (long long)s.k0 * a.ldv + hk * (D * 2);
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
   const Stager<D> sk(a.ldk), sv(a.ldv);
-  auto stage = [&](int n) WIN_INLINE {
+  auto stage = [&](int n, int buf) WIN_INLINE {
     const int j0 = kt.at(n) * TILE;
-    sk(kb + (long long)j0 * a.ldk, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB);
-    sv(vb + (long long)j0 * a.ldv, s.nk - 1 - j0, l0 + (n & 1) * 2 * TB + TB);
+    sk(kb + (long long)j0 * a.ldk, s.nk - 1 - j0, l0 + buf * 2 * TB);
+    sv(vb + (long long)j0 * a.ldv, s.nk - 1 - j0, l0 + buf * 2 * TB + TB);
   };
   const int iw = i0 + wave * 32, i = iw + (lane & 31), ic = min(i, s.nq - 1);
   const int p = ic + off, hi = min(s.nk - 1, p + a.right), lo = p - a.left;
@@ -257,13 +257,12 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[dt][r] = 0.f;
-  if (kt.count) stage(0);
-  for (int n = 0; n < kt.count; ++n) {
+  auto tile = [&](int n, int odd) WIN_INLINE {
     tile_barrier();
-    if (n + 1 < kt.count) stage(n + 1);
+    if (n + 1 < kt.count) stage(n + 1, 1 - odd);
     const int j0 = kt.at(n) * TILE;
-    if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) continue;
-    const char* Kt = lds + (n & 1) * 2 * TB;
+    if (iw >= s.nq || j0 > min(s.nk - 1, wp1 + a.right) || (j0 + TILE - 1 < wp0 - a.left && j0 >= a.sinks)) return;
+    const char* Kt = lds + odd * 2 * TB;
     const char* Vt = Kt + TB;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -275,14 +274,11 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
         st = mfma32<T>(row_frag32<D>(Kt, u * 32, ks), qf[ks], st);
         dp = mfma32<T>(row_frag32<D>(Vt, u * 32, ks), df[ks], dp);
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -lse2));
-        st[r] = pr * (dp[r] - delta);
-      }
       const int ju = j0 + u * 32;
       const bool edge_hi = ju + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = ju < wp1 - a.left && ju + 31 >= a.sinks;
-      if (edge_lo | edge_hi) mask_keys<true>(st, ju + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
+      if (edge_lo | edge_hi) mask_keys(st, ju + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -lse2)) * (dp[r] - delta);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const s16x8 sf = pack8<T>(st, h);
@@ -290,7 +286,14 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
         for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma32<T>(col_frag32<D>(Kt, u * 32 + h * 16, dt), sf, dq[dt]);
       }
     }
+  };
+  if (kt.count) stage(0, 0);
+  int n = 0;
+  for (; n + 1 < kt.count; n += 2) {                                   // two tiles a turn: LDS addresses are constants
+    tile(n, 0);
+    tile(n + 1, 1);
   }
+  if (n < kt.count) tile(n, 0);
   if (i >= s.nq) return;
   char* po = a.dq + row * a.lddq + pl.h * (D * 2);
   typedef __attribute__((ext_vector_type(4))) T T4;
@@ -393,6 +396,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
       }
+      if (iu < flo || iu + 31 > fhi) mask_queries(st, iu + 4 * half, ilo, ihi);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(Lt + u * 32 + 8 * g + 4 * half);
@@ -403,11 +407,6 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
           st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -ls[e]));
           dp[r] -= de[e];
         }
-      }
-      if (iu < flo || iu + 31 > fhi) {
-        const Bounds bd{ilo - iu - 4 * half, ihi - iu - 4 * half, 0};
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
       }
       if (do_v) {
 #pragma unroll
@@ -539,6 +538,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
         st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
         dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
       }
+      if (iu < flo || iu + 31 > fhi) mask_queries(st, iu + 4 * half, ilo, ihi);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(Lt + 8 * g), de = *reinterpret_cast<const f32x4*>(Lt + 64 + 8 * g);
@@ -548,11 +548,6 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
           st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], c, -ls[e]));
           dp[r] -= de[e];
         }
-      }
-      if (iu < flo || iu + 31 > fhi) {
-        const Bounds bd{ilo - iu - 4 * half, ihi - iu - 4 * half, 0};
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = bd.sees(r) ? st[r] : 0.f;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] *= st[r];
