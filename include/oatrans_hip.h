@@ -330,6 +330,17 @@ int oat_attn_window_step(const void* qkv, long long ldqkv, const int* past, void
 int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k, int max_k,
                           void* k_cache, void* v_cache, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream);
 
+/* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
+ * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused), attention with the sequences' query rows as their key rows, out [M, Hq * D]
+ * dense, and - with k_cache - the prompt's cache.  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back; workspace as for
+ * oat_attn_window_bwd with max_q = max_k = longest. */
+int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, const OatRope* rope, const int* pos, int period, void* out, float* lse,
+                             const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks,
+                             float scale, void* k_cache, void* v_cache, const long long* strides, int cap, void* stream);
+int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const OatRope* rope, const int* pos, int period, const void* out,
+                             const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D,
+                             int dtype, int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- input pipeline, device side: decoded frames -> clip tensor.  Replaces, per batch and in one launch,
  * frames.float() / 255 (base/base_dataset.py:519,533,544) and the tensor transforms of data_loader/transforms.py:4-31 /
  * base_dataset_global_local.py:251-257: crop box + bilinear resize (= torchvision Resize on tensors =

@@ -33,30 +33,35 @@ def rope_axes(x, pos, rope, heads, head_dim):
     return _RopeFn.apply(x, pos, rope, heads, head_dim)
 
 
-def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse):
-    """-> (out, turned q | k or None): rotary positions into a new buffer (the values stay where they are), attention over it.  The
-    arguments of both calls are columns of two buffers, checked here once, so the calls get addresses."""
-    M, n = qkv.shape[0], (heads + kv_heads) * D
+def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, cache):
+    """-> (out, turned q | k or None): rotary positions into a new buffer (the values stay where they are), attention over it, and the
+    prompt's rows into the cache, in one call."""
+    M, dev, dt = qkv.shape[0], qkv.device, qkv.dtype
     what = "window_attention"
-    if qkv.stride(1) != 1 or qkv.dtype not in (torch.bfloat16, torch.float16):
+    if qkv.stride(1) != 1 or (dt is not torch.bfloat16 and dt is not torch.float16):
         raise hip.OatError(f"{what}: qkv must be bf16 or fp16 with unit column stride")
-    if seqs.dtype != torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous() or seqs.device != qkv.device:
-        raise hip.OatError(f"{what}: seqs must be a contiguous int32 [B, 4] on {qkv.device}")
-    lib, dtype, base, ld = hip.lib(), hip._ELEMENTS[qkv.dtype], qkv.data_ptr(), hip._ld(qkv)
-    qk, at, ldqk = None, base, ld
+    if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous() or seqs.device != dev:
+        raise hip.OatError(f"{what}: seqs must be a contiguous int32 [B, 4] on {dev}")
+    qk = turned = struct = places = None
+    period = 0
     if rope is not None:
-        if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[1] != rope.axes or not pos.is_contiguous() or pos.device != qkv.device:
-            raise hip.OatError(f"{what}: pos must be a contiguous int32 [P, {rope.axes}] on {qkv.device}")
-        qk = torch.empty(M, n, dtype=qkv.dtype, device=qkv.device)
-        at, ldqk = qk.data_ptr(), n
-        hip._launch(qkv.device, lib.oat_rope_axes, (base, ld, at, n, dtype, pos.data_ptr(), pos.shape[0], M, heads + kv_heads, D, rope.struct, 0),
-                    "oat_rope_axes")
-    out = (torch.empty if packed else torch.zeros)(M, heads * D, dtype=qkv.dtype, device=qkv.device)
-    size = qkv.element_size()
-    hip._launch(qkv.device, lib.oat_attn_window_fwd, (
-        at, ldqk, at + heads * D * size, ldqk, base + n * size, ld, out.data_ptr(), heads * D, lse.data_ptr() if lse is not None else None,
-        seqs.data_ptr(), seqs.shape[0], longest, longest, M, M, heads, kv_heads, D, dtype, *window, D ** -0.5 if scale is None else scale),
-        "oat_attn_window_fwd")
+        if pos.dtype is not torch.int32 or pos.dim() != 2 or pos.shape[1] != rope.axes or not pos.is_contiguous() or pos.device != dev:
+            raise hip.OatError(f"{what}: pos must be a contiguous int32 [P, {rope.axes}] on {dev}")
+        qk = torch.empty(M, (heads + kv_heads) * D, dtype=dt, device=dev)
+        turned, struct, places, period = qk.data_ptr(), rope.struct, pos.data_ptr(), pos.shape[0]
+    out = (torch.empty if packed else torch.zeros)(M, heads * D, dtype=dt, device=dev)
+    kc = vc = strides = None
+    cap = 0
+    if cache is not None:
+        k, v = cache
+        strides, cap = hip._cache_args(k, v, what), k.shape[1]
+        if k.dtype is not dt or k.device != dev or k.shape[0] != seqs.shape[0] or k.shape[2] != kv_heads or k.shape[3] != D:
+            raise hip.OatError(f"{what}: the caches must be [{seqs.shape[0]}, slots, {kv_heads}, {D}] of {dt} on {dev}")
+        kc, vc = k.data_ptr(), v.data_ptr()
+    hip._launch(dev, hip.lib().oat_window_attention_fwd, (
+        qkv.data_ptr(), hip._ld(qkv), turned, struct, places, period, out.data_ptr(), lse.data_ptr() if lse is not None else None,
+        seqs.data_ptr(), seqs.shape[0], longest, M, heads, kv_heads, D, hip._ELEMENTS[dt], *window, D ** -0.5 if scale is None else scale,
+        kc, vc, strides, cap), what)
     return out, qk
 
 
@@ -67,7 +72,7 @@ class _WindowFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed):
         lse = torch.empty(qkv.shape[0], heads, dtype=torch.float32, device=qkv.device)
-        out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse)
+        out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, None)
         ctx.save_for_backward(qkv, qk, out, lse, seqs, pos)
         ctx.args = heads, kv_heads, D, longest, window, scale, rope, packed
         return out
@@ -77,14 +82,16 @@ class _WindowFn(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, qk, out, lse, seqs, pos = ctx.saved_tensors
         heads, kv_heads, D, longest, window, scale, rope, packed = ctx.args
-        n, a = (heads + kv_heads) * D, heads * D
-        qk = qkv if qk is None else qk
-        dqkv = (torch.empty if packed else torch.zeros)(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        hip.attn_window_bwd(qk[:, :a], qk[:, a:n], qkv[:, n:], out, lse, dout.contiguous(), seqs, heads, kv_heads, D, longest, longest, *window,
-                            scale=scale, dq=dqkv[:, :a], dk=dqkv[:, a:n], dv=dqkv[:, n:])
-        if rope is not None:
-            turned = dqkv[:, :n]
-            hip.rope_axes(turned, pos, rope, heads + kv_heads, D, out=turned, inverse=True)
+        dout, dev, lib = dout.contiguous(), qkv.device, hip.lib()
+        M, B = qkv.shape[0], seqs.shape[0]
+        dqkv = (torch.empty if packed else torch.zeros)(qkv.shape, dtype=qkv.dtype, device=dev)
+        need = lib.oat_attn_window_bwd_workspace_bytes(M, B, longest, longest, heads, kv_heads, D, window[0], window[2])
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        hip._launch(dev, lib.oat_window_attention_bwd, (
+            qkv.data_ptr(), hip._ld(qkv), qk.data_ptr() if qk is not None else None, rope.struct if rope is not None else None,
+            pos.data_ptr() if pos is not None else None, pos.shape[0] if pos is not None else 0, out.data_ptr(), lse.data_ptr(),
+            dout.data_ptr(), dqkv.data_ptr(), seqs.data_ptr(), B, longest, M, heads, kv_heads, D, hip._ELEMENTS[qkv.dtype], *window,
+            D ** -0.5 if scale is None else scale, ws.data_ptr(), need), "window_attention backward")
         return dqkv, None, None, None, None, None, None, None, None, None, None
 
 
@@ -109,17 +116,12 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
         return _WindowFn.apply(qkv, seqs, pos, heads, kv_heads, D, longest, (left, right, sinks), scale, rope, packed)
     if grad:
         raise hip.OatError("window_attention: a cache takes a prompt without a gradient (use torch.no_grad())")
-    qkv = qkv.detach()
     if cache is not None:
         slots = cache[0].shape[1]
         if right != 0 or (slots < longest and not (left >= 0 and slots == sinks + left + 1)):
             raise hip.OatError("window_attention: a cache belongs to causal attention (right = 0) and needs a slot for every token, or "
                                "sinks + left + 1 slots")
-    out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, (left, right, sinks), scale, rope, packed, None)
-    if cache is not None:
-        n = (heads + kv_heads) * D
-        hip.window_cache_fill((qkv if qk is None else qk)[:, heads * D:n], qkv[:, n:], seqs, cache[0], cache[1], longest, sinks=sinks)
-    return out
+    return _forward(qkv, seqs, pos, heads, kv_heads, D, longest, (left, right, sinks), scale, rope, packed, None, cache)[0]
 
 
 class WindowCache:

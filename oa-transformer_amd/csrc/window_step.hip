@@ -407,3 +407,45 @@ extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v
   OAT_LAUNCH(cache_fill_kernel, dim3((unsigned)min((n + 255) / 256, 4096ll), B), dim3(256), 0, (hipStream_t)stream, a);
   return check_launch(me);
 }
+
+// ---- what a layer on packed q | k | v rows does, in one call each way (one crossing into the library instead of three)
+static int packed_wrong(const char* me, const OatRope* rope, const void* turned, int M, int Hq, int Hkv) {
+  if (rope && !turned) return fail(me, "rotary positions need a buffer for the turned queries and keys");
+  if (M < 0 || Hq < 1 || Hkv < 1) return fail(me, "no heads, or a negative number of rows");
+  return 0;
+}
+
+extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, const OatRope* rope, const int* pos, int period, void* out,
+                                        float* lse, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left,
+                                        int right, int sinks, float scale, void* kc, void* vc, const long long* strides, int cap, void* stream) {
+  if (int rc = packed_wrong("window_attention_fwd", rope, turned, M, Hq, Hkv)) return rc;
+  const long long n = (long long)(Hq + Hkv) * D, a = (long long)Hq * D;
+  const char* q = (const char*)qkv;
+  const char* v = M ? q + n * 2 : q;
+  long long ldq = ld;
+  if (rope) {
+    if (int rc = oat_rope_axes(qkv, ld, turned, n, dtype, pos, period, M, Hq + Hkv, D, rope, 0, stream)) return rc;
+    q = (const char*)turned;
+    ldq = n;
+  }
+  const char* k = M ? q + a * 2 : q;
+  if (int rc = oat_attn_window_fwd(q, ldq, k, ldq, v, ld, out, a, lse, seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks,
+                                   scale, stream)) return rc;
+  return kc ? oat_window_cache_fill(k, ldq, v, ld, seqs, B, M, longest, kc, vc, strides, cap, Hkv, D, sinks, stream) : 0;
+}
+
+extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const OatRope* rope, const int* pos, int period,
+                                        const void* out, const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest,
+                                        int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  if (int rc = packed_wrong("window_attention_bwd", rope, turned, M, Hq, Hkv)) return rc;
+  if (M == 0) return 0;
+  const long long n = (long long)(Hq + Hkv) * D, a = (long long)Hq * D, w = n + (long long)Hkv * D;
+  const char* q = (const char*)(rope ? turned : qkv);
+  const long long ldq = rope ? n : ld;
+  char* g = (char*)dqkv;
+  if (int rc = oat_attn_window_bwd(q, ldq, q + a * 2, ldq, (const char*)qkv + n * 2, ld, out, a, lse, dout, a, g, w, g + a * 2, w, g + n * 2, w,
+                                   seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes,
+                                   stream)) return rc;
+  return rope ? oat_rope_axes(g, w, g, w, dtype, pos, period, M, Hq + Hkv, D, rope, 1, stream) : 0;
+}
