@@ -83,6 +83,8 @@ class _WindowFn(torch.autograd.Function):
         qkv, qk, out, lse, seqs, pos = ctx.saved_tensors
         heads, kv_heads, D, longest, window, scale, rope, packed = ctx.args
         dout, dev, lib = dout.contiguous(), qkv.device, hip.lib()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
         M, B = qkv.shape[0], seqs.shape[0]
         dqkv = (torch.empty if packed else torch.zeros)(qkv.shape, dtype=qkv.dtype, device=dev)
         need = lib.oat_attn_window_bwd_workspace_bytes(M, B, longest, longest, heads, kv_heads, D, window[0], window[2])

@@ -6,6 +6,7 @@ every parity claim).  ``import torch`` must happen before the library is loaded
 so that it binds to the HIP runtime torch already mapped (same soname).
 """
 import ctypes
+import functools
 import os
 import re
 
@@ -1148,12 +1149,17 @@ def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, ma
     return dq, dk, dv
 
 
+@functools.lru_cache(maxsize=256)
+def _six(*strides):
+    return (_L * 6)(*strides)
+
+
 def _cache_args(k_cache, v_cache, what):
-    ok = (k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.device == v_cache.device
-          and k_cache.dtype in (torch.bfloat16, torch.float16) and k_cache.stride(3) == v_cache.stride(3) == 1)
-    if not ok:
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if (len(ks) != 4 or v_cache.shape != k_cache.shape or ks[3] != 1 or vs[3] != 1 or k_cache.dtype != v_cache.dtype
+            or k_cache.dtype not in (torch.bfloat16, torch.float16) or k_cache.device != v_cache.device):
         raise OatError(f"{what}: the caches must be [B, slots, heads, head_dim] of bf16 or fp16, both alike, with unit last stride")
-    return (_L * 6)(*k_cache.stride()[:3], *v_cache.stride()[:3])
+    return _six(*ks[:3], *vs[:3])
 
 
 def window_step_workspace(B, heads, kv_heads, head_dim, device="cuda"):

@@ -266,6 +266,11 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
     const char* Vt = Kt + TB;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      const int ju = j0 + u * 32;
+      // 32 keys that no query of the wave sees.  Heads of 64 look at both halves of a tile together: without a branch between them the
+      // compiler lays one half's products beside the other's exponentials (two 16-frame clips 139 us, with a branch 143; heads of 128,
+      // where the registers do not allow that: six packed texts 82 us without this one, 79 with it)
+      if (D == 128 && (ju > min(s.nk - 1, wp1 + a.right) || (ju + 31 < wp0 - a.left && ju >= a.sinks))) continue;
       f32x16 st, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
@@ -274,7 +279,6 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
         st = mfma32<T>(row_frag32<D>(Kt, u * 32, ks), qf[ks], st);
         dp = mfma32<T>(row_frag32<D>(Vt, u * 32, ks), df[ks], dp);
       }
-      const int ju = j0 + u * 32;
       const bool edge_hi = ju + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = ju < wp1 - a.left && ju + 31 >= a.sinks;
       if (edge_lo | edge_hi) mask_keys(st, ju + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
 #pragma unroll
