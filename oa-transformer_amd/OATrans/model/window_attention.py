@@ -105,6 +105,8 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
     token j if j <= i + right and (j >= i - left or j < sinks); left / right < 0: no such edge, right = 0: causal.
     rope, pos: rotary positions of q and k, pos int32 [P, axes] with M a multiple of P.
     packed: the caller states that every row belongs to a sequence; otherwise rows of none (padding) get zeros, and zero gradients.
+    Rows of no sequence may hold anything; rows of a sequence have to be finite (a masked pair's weight is an exact zero, and it is
+    multiplied).
     cache: (k, v) of [B, slots, kv_heads, head_dim] that take the prompt's turned keys and its values (no gradient then); fewer slots
     than tokens only where they are the sinks and the window, sinks + left + 1."""
     D = head_dim
@@ -112,7 +114,8 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
         raise hip.OatError(f"window_attention: qkv must be [M, {(heads + 2 * kv_heads) * D}]")
     if (rope is None) != (pos is None):
         raise hip.OatError("window_attention: rope and pos belong together")
-    longest = qkv.shape[0] if longest is None else int(longest)
+    longest = qkv.shape[0] if longest is None else min(int(longest), qkv.shape[0])
+    left, right, sinks = hip._reach(left), hip._reach(right), hip._reach(sinks)
     grad = torch.is_grad_enabled() and qkv.requires_grad
     if cache is None and grad:
         return _WindowFn.apply(qkv, seqs, pos, heads, kv_heads, D, longest, (left, right, sinks), scale, rope, packed)

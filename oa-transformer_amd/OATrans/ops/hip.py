@@ -1047,6 +1047,11 @@ def _rows(t, columns, dtype, device, what):
                        f"on {t.device}, strides {t.stride()}")
 
 
+def _reach(n):
+    """a window's side or its sinks as the library's int: what is further than any token is 2^29"""
+    return n if -1 <= n <= 1 << 29 else -1 if n < 0 else 1 << 29
+
+
 def _ld(t):
     # (a matrix of one row may carry any row stride, and never uses it)
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -1091,7 +1096,7 @@ def seq_table(q_lens, k_lens=None, q_rows=None, k_rows=None, device="cuda"):
     return torch.tensor(list(zip(q_rows, q_lens, k_rows, k_lens)), dtype=torch.int32).reshape(-1, 4).to(device)
 
 
-def _window_args(q, k, v, seqs, heads, kv_heads, D, what):
+def _window_args(q, k, v, seqs, heads, kv_heads, D, max_q, max_k, what):
     _need(q.dtype in (torch.bfloat16, torch.float16), f"{what}: q, k, v must be bf16 or fp16")
     _rows(q, heads * D, q.dtype, q.device, f"{what}: q")
     _rows(k, kv_heads * D, q.dtype, q.device, f"{what}: k")
@@ -1099,13 +1104,14 @@ def _window_args(q, k, v, seqs, heads, kv_heads, D, what):
     _need(k.shape[0] == v.shape[0], f"{what}: k and v have different numbers of rows")
     _need(seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[1] == 4 and seqs.is_contiguous() and seqs.device == q.device,
           f"{what}: seqs must be a contiguous int32 [B, 4] on {q.device}")
+    _need(0 <= max_q <= 1 << 29 and 0 <= max_k <= 1 << 29, f"{what}: the largest counts are 0 to 2^29")
 
 
 def attn_window_fwd(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, left=-1, right=0, sinks=0, scale=None, out=None, lse=None):
     """out [rows, heads * head_dim] = attention of q over k, v within a sliding window with sinks (see oat_attn_window_fwd).
     seqs: int32 [B, 4] on the device (seq_table); max_q / max_k: the largest counts in it.  lse: fp32 [rows, heads], written where
     given (the backward pass needs it).  A new `out` starts as zeros, a given one keeps its rows of no sequence."""
-    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, "attn_window_fwd")
+    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, "attn_window_fwd")
     if out is None:
         out = torch.zeros(q.shape[0], heads * head_dim, dtype=q.dtype, device=q.device)
     _rows(out, heads * head_dim, q.dtype, q.device, "attn_window_fwd: out")
@@ -1114,8 +1120,8 @@ def attn_window_fwd(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, left
           "attn_window_fwd: lse must be a contiguous fp32 [rows, heads]")
     _launch(q.device, lib().oat_attn_window_fwd, (
         q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr() if lse is not None else None,
-        seqs.data_ptr(), seqs.shape[0], max_q, max_k, q.shape[0], k.shape[0], heads, kv_heads, head_dim, _ELEMENTS[q.dtype], left, right,
-        sinks, head_dim ** -0.5 if scale is None else scale), "oat_attn_window_fwd")
+        seqs.data_ptr(), seqs.shape[0], max_q, max_k, q.shape[0], k.shape[0], heads, kv_heads, head_dim, _ELEMENTS[q.dtype], _reach(left),
+        _reach(right), _reach(sinks), head_dim ** -0.5 if scale is None else scale), "oat_attn_window_fwd")
     return out
 
 
@@ -1124,7 +1130,7 @@ def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, ma
     """(dq, dk, dv) of attn_window_fwd.  New outputs start as zeros, given ones keep their rows of no sequence.  workspace: fp32 of
     oat_attn_window_bwd_workspace_bytes(...) bytes (default: a new one)."""
     what = "attn_window_bwd"
-    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, what)
+    _window_args(q, k, v, seqs, heads, kv_heads, head_dim, max_q, max_k, what)
     D, dt, dev, M = head_dim, q.dtype, q.device, q.shape[0]
     _rows(out, heads * D, dt, dev, what + ": out")
     _rows(dout, heads * D, dt, dev, what + ": dout")
@@ -1139,12 +1145,13 @@ def attn_window_bwd(q, k, v, out, lse, dout, seqs, heads, kv_heads, head_dim, ma
     _rows(dv, kv_heads * D, dt, dev, what + ": dv")
     _need(dq.shape[0] == M and dk.shape[0] == dv.shape[0] == k.shape[0], what + ": dq, dk, dv have as many rows as q, k, v")
     if workspace is None:
-        workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, seqs.shape[0], max_q, max_k, heads, kv_heads, D, left, sinks) // 4, dtype=torch.float32, device=dev)
+        workspace = torch.empty(lib().oat_attn_window_bwd_workspace_bytes(M, seqs.shape[0], max_q, max_k, heads, kv_heads, D, _reach(left),
+                                                                            _reach(sinks)) // 4, dtype=torch.float32, device=dev)
     _need(workspace.is_contiguous() and workspace.device == dev, what + ": workspace must be contiguous on the same device")
     _launch(dev, lib().oat_attn_window_bwd, (
         q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out), lse.data_ptr(), dout.data_ptr(), _ld(dout),
         dq.data_ptr(), _ld(dq), dk.data_ptr(), _ld(dk), dv.data_ptr(), _ld(dv), seqs.data_ptr(), seqs.shape[0], max_q, max_k, M, k.shape[0],
-        heads, kv_heads, D, _ELEMENTS[dt], left, right, sinks, D ** -0.5 if scale is None else scale, workspace.data_ptr(),
+        heads, kv_heads, D, _ELEMENTS[dt], _reach(left), _reach(right), _reach(sinks), D ** -0.5 if scale is None else scale, workspace.data_ptr(),
         workspace.numel() * workspace.element_size()), "oat_attn_window_bwd")
     return dq, dk, dv
 
@@ -1163,7 +1170,8 @@ def _cache_args(k_cache, v_cache, what):
 
 
 def window_step_workspace(B, heads, kv_heads, head_dim, device="cuda"):
-    """The zeroed workspace of attn_window_step (its contents belong to the operator; steps that may run at once need one each)."""
+    """The zeroed workspace of attn_window_step for these sizes (its contents belong to the operator; steps that may run at once need
+    one each, and so do steps of other sizes)."""
     return torch.zeros(lib().oat_attn_window_step_workspace_bytes(B, heads, kv_heads, head_dim) // 4, dtype=torch.float32, device=device)
 
 
@@ -1192,7 +1200,7 @@ def attn_window_step(qkv, past, k_cache, v_cache, heads, left=-1, sinks=0, rolli
         _need(out.shape[0] == B, what + ": one row of out per sequence")
     _launch(dev, lib().oat_attn_window_step, (
         qkv.data_ptr(), _ld(qkv), past.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, cap, out.data_ptr(), _ld(out), B, heads,
-        kv_heads, D, _ELEMENTS[dt], left, sinks, int(rolling), D ** -0.5 if scale is None else scale,
+        kv_heads, D, _ELEMENTS[dt], _reach(left), _reach(sinks), int(rolling), D ** -0.5 if scale is None else scale,
         rope.struct if rope is not None else None, pos.data_ptr() if rope is not None else None, pieces.data_ptr(),
         pieces.numel() * pieces.element_size()), "oat_attn_window_step")
     return out
@@ -1207,6 +1215,7 @@ def window_cache_fill(k, v, seqs, k_cache, v_cache, max_k, sinks=0):
     _rows(v, kv_heads * D, k_cache.dtype, k_cache.device, what + ": v")
     _need(k.shape[0] == v.shape[0], what + ": k and v have different numbers of rows")
     _need(seqs.dtype == torch.int32 and seqs.shape == (B, 4) and seqs.is_contiguous() and seqs.device == k.device, what + ": seqs must be int32 [B, 4]")
+    _need(0 <= max_k <= 1 << 29, what + ": the largest count is 0 to 2^29")
     _launch(k.device, lib().oat_window_cache_fill, (
         k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), seqs.data_ptr(), B, k.shape[0], max_k, k_cache.data_ptr(), v_cache.data_ptr(), strides,
-        cap, kv_heads, D, sinks), "oat_window_cache_fill")
+        cap, kv_heads, D, _reach(sinks)), "oat_window_cache_fill")

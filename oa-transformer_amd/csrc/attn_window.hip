@@ -8,6 +8,11 @@ namespace oat {
 //     S^T = K Q^T      P^T = exp2(c S^T - c m)      O^T += V^T P^T       c = scale log2(e), m = running maximum of the row
 // The query is the COLUMN of S^T: a lane holds 16 of 32 keys of ONE query, so maximum and sum of a row are register work and one
 // exchange with lane ^ 32, and P^T is the B operand of the second product where it stands.
+// Bound: instruction issue.  The 32 keys of a step are 8 matrix instructions (heads of 64) and about 130 vector ones; two waves of a SIMD
+// take 293 clocks for the first alone, 313 for the second alone, 440 for both: the two units overlap for a third of it.  128 queries
+// share each staged tile, so the LDS and HBM are idle most of the time.  Measured: two clips of 7057 tokens (12 heads of 64, window of
+// 882 to each side) 108 us = 665 TFLOP/s; 8191 tokens (32 / 8 heads of 128, causal, window of 1024) 174 us = 743; six packed texts of
+// 512 to 2048 (16 / 4 heads of 128, window of 512) 66 us = 418: a fourth of the products there are masked at the window's edges.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
@@ -202,7 +207,8 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
 // Two kernels that form S and dO V^T again, one over queries (dQ), one over keys (dK, dV; the query heads that share a key head are
 // summed in the workgroup): 7 products for the 5 of one kernel with atomic sums, but every sum has one fixed order.
 
-// dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
+// dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  Bound: instruction issue, as above, with three products
+// for one exponential: the clips of above 139 us = 775 TFLOP/s, the packed texts 80 us = 517.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
@@ -313,7 +319,8 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
 }
 
 // dK and dV of 128 keys (32 a wave): S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and
-// their gradients pass through the LDS in tiles of 64, with their lse2 and delta.
+// their gradients pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: instruction issue (four products for one
+// exponential): the clips of above 180 us = 797 TFLOP/s.
 //
 // The sinks' keys are seen by every later query: one workgroup would walk the whole sequence while the others walk a window.  So the
 // pairs beyond the window (the far ones) get workgroups of their own: 32 sink keys and one of `pieces` shares of the far queries each,
@@ -462,9 +469,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
     }
 }
 
-// The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other through the LDS, and then one adds
-// up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum instead of two (64 instead of 128
-// registers at D = 128), so that two waves fit a SIMD.
+// The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other
+// through the LDS, and then one adds up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum
+// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above: 111 us = 497 TFLOP/s.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
@@ -645,6 +652,7 @@ static FarSplit far_split(int B, int Hq, int Hkv, int D, int max_q, int max_k, i
   const long long rows = min((long long)max_q, (long long)max_k - left);
   if (sinks < 1 || min(sinks, max_k) > 512 || rows <= 512 || B < 1) return {0, 0};
   const int groups = (min(sinks, max_k) + 31) / 32;
+  if ((long long)B * Hkv * groups * (2 * D / 8) >= 1ll << 24) return {0, 0};              // (win_bwd_sink_kernel: a launch holds 2^32 threads)
   // as many workgroups as stay resident: two a CU with heads of 64, one with heads of 128
   const long long want = (D == 64 ? 512 : 256) / max(1ll, (long long)B * Hkv * groups);
   return {groups, (int)max(1ll, min(want, rows * (Hq / Hkv) / 256))};
@@ -743,7 +751,7 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
     set_error("attn_window_bwd: k, v, dk, dv need 16-byte aligned rows (pitch a multiple of 8, at least the heads, at most 2^22 values)");
     return -2;
   }
-  if (rows_q && (!workspace || workspace_bytes < oat_attn_window_bwd_workspace_bytes(rows_q, B, max_q, max_k, Hq, Hkv, D, left, sinks))) { set_error("attn_window_bwd: the workspace is too small"); return -3; }
+  if (rows_q && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < oat_attn_window_bwd_workspace_bytes(rows_q, B, max_q, max_k, Hq, Hkv, D, left, sinks))) { set_error("attn_window_bwd: the workspace is too small, or not aligned to 16 bytes"); return -3; }
   WinArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)out; a.dout = (const char*)dout;
   a.lse = const_cast<float*>(lse); a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;

@@ -49,6 +49,8 @@ template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
 // The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
 // new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in a fixed order.
+// Measured: 64 sequences of up to 4096 tokens, 32 / 8 heads of 128: 576 MB in 114 us = 5.0 TB/s; two of 65536 visible tokens: 537 MB in
+// 104 us = 5.1 (a large copy: 4.9 to 5.4); one of 512, 12 heads of 64: 7.7 us, a chain of dependent loads.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -354,8 +356,9 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
     if (const char* w = rope_wrong(rope, D)) return fail(me, w);
     if (!pos) return fail(me, "positions are needed to turn by");
   }
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < oat_attn_window_step_workspace_bytes(B, Hq, Hkv, D))
-    return fail(me, "the workspace is too small, or not aligned to 16 bytes");
+  // (of other sizes its tickets would stand elsewhere, where this call's may find sums instead of zeros)
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes != oat_attn_window_step_workspace_bytes(B, Hq, Hkv, D))
+    return fail(me, "the workspace is not one of these sizes (B, Hq, Hkv, D), or not aligned to 16 bytes");
   if ((long long)B * Hkv * ((Hq / Hkv + 15) / 16) * most_pieces(B, Hkv) >= (1ll << 23)) return fail(me, "more than 2^23 pieces");
   StepArgs a{};
   a.qkv = (const char*)qkv; a.ldqkv = ldqkv * 2; a.past = past; a.pos = pos;
@@ -410,7 +413,7 @@ extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v
 
 // ---- what a layer on packed q | k | v rows does, in one call each way (one crossing into the library instead of three)
 static int packed_wrong(const char* me, const OatRope* rope, const void* turned, int M, int Hq, int Hkv) {
-  if (rope && !turned) return fail(me, "rotary positions need a buffer for the turned queries and keys");
+  if (rope && !turned && M) return fail(me, "rotary positions need a buffer for the turned queries and keys");
   if (M < 0 || Hq < 1 || Hkv < 1) return fail(me, "no heads, or a negative number of rows");
   return 0;
 }

@@ -173,3 +173,39 @@ def test_oracle_of_the_window_against_dense_attention():
     pos = torch.tensor([[1, 5], [0, 0], [7, 2]])
     y = wo.rope(x, pos, (4, 4), 50.0)
     assert torch.allclose(wo.rope(y, pos, (4, 4), 50.0, inverse=True), x) and torch.allclose(y[1], x[1]) and torch.allclose(y.norm(dim=-1), x.norm(dim=-1))
+
+
+LAYER = dict(qkv=4096, ld=256, turned=None, rope=None, pos=None, period=0, out=4096, lse=None, seqs=4096, B=1, longest=10, M=10, Hq=2, Hkv=1, D=64,
+             dtype=0, left=-1, right=0, sinks=0, scale=0.125, kc=None, vc=None, strides=None, cap=0)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(D=96), b"64 or 128"), (dict(dtype=2), b"element type"), (dict(Hq=3, Hkv=2), b"multiple"), (dict(Hkv=0), b"no heads"), (dict(M=-1), b"no heads"),
+    (dict(longest=2 ** 30), b"lengths"), (dict(seqs=None), b"table"), (dict(sinks=-1), b"sinks"), (dict(scale=0.0), b"scale"), (dict(qkv=4098), b"16-byte"),
+    (dict(ld=248, D=128), b"16-byte"), (dict(rope=True, pos=4096, period=10), b"turned"), (dict(rope=True, turned=4096, period=10), b"needed"),
+    (dict(rope=True, turned=4096, pos=4096, period=3), b"whole number")])
+def test_layer_refusals(change, text):
+    hip = _hip()
+    a = {**LAYER, **change}
+    if a["rope"]:
+        a["rope"] = hip.RopeAxes((64,)).struct
+    _refused(hip, hip.lib().oat_window_attention_fwd(*a.values(), None), text)
+    if "period" in change and text != b"turned":                   # (the way back turns last: its rotary arguments are the forward's)
+        return
+    head = [a[n] for n in ("qkv", "ld", "turned", "rope", "pos", "period", "out")] + [4096, 4096, 4096]
+    tail = [a[n] for n in ("seqs", "B", "longest", "M", "Hq", "Hkv", "D", "dtype", "left", "right", "sinks", "scale")]
+    _refused(hip, hip.lib().oat_window_attention_bwd(*head, *tail, 4096, 1 << 40, None), text)
+
+
+def test_workspaces_belong_to_their_sizes():
+    hip = _hip()
+    a = {**STEP, "strides": (LL * 6)(*STEP["strides"])}
+    need = hip.lib().oat_attn_window_step_workspace_bytes(1, 2, 1, 64)
+    for n in (need - 4, need + 4, hip.lib().oat_attn_window_step_workspace_bytes(2, 2, 1, 64)):
+        _refused(hip, hip.lib().oat_attn_window_step(*{**a, "n": n}.values(), None), b"workspace")
+    _refused(hip, hip.lib().oat_attn_window_step(*{**a, "n": need, "ws": 4100}.values(), None), b"workspace")
+    q = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for most in (-1, 2 ** 29 + 1, 2 ** 32 + 4):                    # a count is not cut to its low 32 bits
+        with pytest.raises(hip.OatError, match="largest counts"):
+            hip.attn_window_fwd(q, q, q, hip.seq_table([4], device="cpu"), 1, 1, 64, most, 4)
+    assert [hip._reach(n) for n in (-7, -1, 0, 9, 2 ** 29, 2 ** 29 + 1, 2 ** 32, 2 ** 63)] == [-1, -1, 0, 9] + [2 ** 29] * 4

@@ -544,3 +544,24 @@ def test_launch_tape_replays_the_operators():
     hip.tape_replay(tape)
     assert torch.equal(out, ref)
     hip.tape_free(tape)
+
+
+def test_reaches_beyond_32_bits_and_counts_beyond_the_rows():
+    """A window, sinks or `longest` larger than anything there is the same as one that just covers it."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    M = 150
+    qkv, seqs = rnd(M, 192), hip.seq_table([M])
+    full = wa.window_attention(qkv, seqs, 1, 1, 64, left=-1, right=-1, longest=M)
+    causal = wa.window_attention(qkv, seqs, 1, 1, 64, left=-1, right=0, longest=M)
+    for far in (M, 2 ** 29 + 7, 2 ** 32, 2 ** 33 + 5):
+        assert torch.equal(wa.window_attention(qkv, seqs, 1, 1, 64, left=far, right=far, longest=far), full)
+        assert torch.equal(hip.attn_window_fwd(qkv[:, :64], qkv[:, 64:128], qkv[:, 128:], seqs, 1, 1, 64, M, M, left=far, right=0), causal)
+        # (other tiles, another reference: each side rounds its weights and its output, u sum P |v| + u |out|)
+        sunk = wa.window_attention(qkv, seqs, 1, 1, 64, left=3, right=0, sinks=far)
+        within(sunk, causal.double(), 4 * half_step(BF) * (causal.double().abs() + qkv[:, 128:].double().abs().max()), "sinks")
+    rope, none = hip.RopeAxes((64,)), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    empty = rnd(0, 192).requires_grad_()
+    out = wa.window_attention(empty, hip.seq_table([0]), 1, 1, 64, rope=rope, pos=none)
+    out.sum().backward()
+    assert out.shape == (0, 64) and empty.grad.shape == (0, 192)
