@@ -124,7 +124,7 @@ struct WinArgs {
   float* slabs;                         // backward: the sinks' sums (win_bwd_kv_kernel)
   int B, Hq, Hkv, left, right, sinks, max_q, max_k, rows_q, rows_k;
   int run;                              // tiles that go to one XCD together
-  int groups, pieces;                   // how the sinks' far queries are split
+  int groups, pieces, far_blocks;       // how the sinks' far queries are split; their workgroups in the launch
   float scale;
 };
 struct Seq { int q0, nq, k0, nk; };

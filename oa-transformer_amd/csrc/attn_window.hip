@@ -318,78 +318,149 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
     }
 }
 
-// dK and dV of 128 keys (32 a wave): S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and
-// their gradients pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: instruction issue (four products for one
-// exponential): the clips of above 180 us = 797 TFLOP/s.
-//
-// The sinks' keys are seen by every later query: one workgroup would walk the whole sequence while the others walk a window.  So the
-// pairs beyond the window (the far ones) get workgroups of their own: 32 sink keys and one of `pieces` shares of the far queries each,
-// where waves 0, 1 form dV and waves 2, 3 dK of the tile's two halves.  Those sums, and what the window gives the sinks, go to 32-bit
-// slabs that win_bwd_sink_kernel adds in a fixed order.
-template <class T, int D, bool far>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArgs a) {
-  constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * ST];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
-  Place pl;
-  int piece = 0, group = 0;
-  if constexpr (far) {
-    const int i = blockIdx.x;
-    if (i >= a.B * a.Hkv * a.groups * a.pieces) return;
-    piece = i % a.pieces;
-    group = i / a.pieces % a.groups;
-    pl.h = i / a.pieces / a.groups % a.Hkv;
-    pl.b = i / a.pieces / a.groups / a.Hkv;
-  } else {
-    if (!place(a, (a.max_k + 127) / 128, a.Hkv, pl)) return;
+// a tile of 64 queries of head h, with their gradients, lse2 and delta, into the LDS
+template <int D> OAT_DEV void stage_queries(const WinArgs& a, const Seq& s, const Stager<D>& sq, const Stager<D>& sd, int h, int t, uint32_t l, int wave) {
+  const int i0 = t * TILE, last = s.nq - 1 - i0;
+  const long long row = s.q0 + i0;
+  sq(a.q + row * a.ldq + h * (D * 2), last, l);
+  sd(a.dout + row * a.lddo + h * (D * 2), last, l + TILE * D * 2);
+  if (wave < 2) {
+    const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 : : "v"((uint32_t)min((int)(threadIdx.x & 63), last) * 4u), "s"(src), "s"(__builtin_amdgcn_readfirstlane(l + 2 * TILE * D * 2 + wave * 256)) : "memory", "m0");
   }
-  const Seq s = load_seq(a, pl.b);
-  const int j0 = far ? group * 32 : pl.tile * 128;
-  if (j0 >= s.nk || (far && j0 >= a.sinks)) return;
-  const int off = s.nk - s.nq, split = a.groups > 0;
-  // the queries that see key j: i = lo(j) .. hi(j)
-  auto lo = [&](int j) WIN_INLINE { return far ? j + a.left - off + 1 : j - a.right - off; };
-  auto hi = [&](int j) WIN_INLINE { return far ? (j < a.sinks ? s.nq - 1 : -1) : !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
-  const int jend = min(j0 + (far ? 31 : 127), s.nk - 1);
-  const int i0 = max(0, lo(j0)), i1 = far || (!split && j0 < a.sinks) ? s.nq - 1 : hi(jend);
-  const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1;
-  const int na = far ? (int)((long long)nt * G * piece / a.pieces) : 0, nb = far ? (int)((long long)nt * G * (piece + 1) / a.pieces) : nt * G;
+}
+// a slab: [dK, dV][D][32 keys]; slots of 32 sinks: (piece, half of its tiles), last the window's own
+template <int D> OAT_DEV float* slab(const WinArgs& a, int b, int hk, int group, int slot, bool is_v) {
+  return a.slabs + ((((size_t)(b * a.Hkv + hk) * a.groups + group) * (2 * a.pieces + 1) + slot) * 2 + is_v) * (D * 32);
+}
+
+// dK and dV: one launch of two kinds of workgroups.
+//
+// The sinks' keys are seen by every later query: the workgroup that owns them would walk the whole sequence while the others walk a
+// window.  So the pairs beyond the window (the far ones) are taken by workgroups of their own (far_keys): 32 sink keys and one of
+// `pieces` shares of the far queries each, where waves 0, 1 form dV and waves 2, 3 dK of the tile's two halves.  Those sums, and what
+// the window gives the sinks, go to 32-bit slabs that win_bwd_sink_kernel adds in a fixed order.  The far workgroups are short and come
+// last in the launch, where they fill its end: two clips of 7057 tokens 179 us for all of it, six packed texts 115; in a launch of their
+// own 184 + 16 and 112 + 24, first in the launch 179 and 129.
+template <class T, int D> OAT_DEV void far_keys(const WinArgs& a, char* lds, int block) {
+  constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
+  const int piece = block % a.pieces, bhg = block / a.pieces, group = bhg % a.groups, hk = bhg / a.groups % a.Hkv, b = bhg / a.groups / a.Hkv;
+  const Seq s = load_seq(a, b);
+  const int j0 = group * 32;
+  if (j0 >= s.nk || j0 >= a.sinks) return;
+  const int off = s.nk - s.nq, j = j0 + (lane & 31), jc = min(j, s.nk - 1), jend = min(j0 + 31, s.nk - 1);
+  // key j is seen from beyond its window by queries lo(j) .. the last
+  auto lo = [&](int j) WIN_INLINE { return j + a.left - off + 1; };
+  const int i0 = max(0, lo(j0)), t0 = i0 / TILE, nt = s.nq - 1 < i0 ? 0 : (s.nq - 1) / TILE - t0 + 1;
+  const int na = __builtin_amdgcn_readfirstlane((int)((long long)nt * G * piece / a.pieces));
+  const int nb = __builtin_amdgcn_readfirstlane((int)((long long)nt * G * (piece + 1) / a.pieces));
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
   const Stager<D> sq(a.ldq), sd(a.lddo);
-  auto stage = [&](int n) WIN_INLINE {
-    const int g = n / nt, i0 = (t0 + n - g * nt) * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
-    const long long row = s.q0 + i0;
-    const uint32_t l = l0 + (n & 1) * ST;
-    sq(a.q + row * a.ldq + h * (D * 2), last, l);
-    sd(a.dout + row * a.lddo + h * (D * 2), last, l + TB);
-    if (wave < 2) {
-      const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
-      const uint32_t dst = l + 2 * TB + wave * 256;
-      uint32_t keep;
-      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-                   : "=&s"(keep) : "v"((uint32_t)min(lane, last) * 4u), "s"(src), "s"(dst) : "memory");
+  auto stage = [&](int n) WIN_INLINE { stage_queries<D>(a, s, sq, sd, hk * G + n / nt, t0 + n % nt, l0 + (n & 1) * ST, wave); };
+  const float c = a.scale * LOG2E;
+  s16x8 kf[D / 16], vf[D / 16];
+  load_cols<D>(kf, a.k + (long long)(s.k0 + jc) * a.ldk + hk * (D * 2));
+  load_cols<D>(vf, a.v + (long long)(s.k0 + jc) * a.ldv + hk * (D * 2));
+  const int ilo = lo(j), ihi = j < min(s.nk, a.sinks) ? s.nq - 1 : -1;
+  const bool do_k = wave >= 2, all_sinks = jend < a.sinks;
+  const int u = wave & 1;
+  f32x16 sum[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[dt][r] = 0.f;
+  if (na < nb) stage(na);
+  for (int n = na; n < nb; ++n) {
+    tile_barrier();
+    if (n + 1 < nb) stage(n + 1);
+    const int iu = (t0 + n % nt) * TILE + u * 32;
+    if (iu >= s.nq || iu + 31 < i0) continue;
+    const char* Qt = lds + (n & 1) * ST;
+    const char* Dt = Qt + TB;
+    const float* Lt = reinterpret_cast<const float*>(Dt + TB) + u * 32 + 4 * half;
+    f32x16 st;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
+    if (iu < lo(jend) || iu + 31 >= s.nq || !all_sinks) mask_queries(st, iu + 4 * half, ilo, ihi);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 ls = *reinterpret_cast<const f32x4*>(Lt + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[4 * g + e], c, -ls[e]));
     }
-  };
-  const int jw = far ? j0 : j0 + wave * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1), jwe = min(jw + 31, s.nk - 1);
+    if (do_k) {
+      f32x16 dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 de = *reinterpret_cast<const f32x4*>(Lt + 64 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[4 * g + e] *= dp[4 * g + e] - de[e];
+      }
+    }
+    const char* Xt = do_k ? Qt : Dt;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const s16x8 f = pack8<T>(st, h);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) sum[dt] = mfma32<T>(col_frag32<D>(Xt, u * 32 + h * 16, dt), f, sum[dt]);
+    }
+  }
+  float* sl = slab<D>(a, b, hk, group, 2 * piece + u, !do_k) + (lane & 31);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sl[(dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3)) * 32] = sum[dt][r];
+}
+
+// 128 keys, 32 a wave: S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and their gradients
+// pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: instruction issue (four products for one exponential): the
+// clips of above 180 us = 797 TFLOP/s.
+template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) {
+  constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
+  Place pl;
+  if (!place(a, (a.max_k + 127) / 128, a.Hkv, pl)) return;
+  const Seq s = load_seq(a, pl.b);
+  const int j0 = pl.tile * 128;
+  if (j0 >= s.nk) return;
+  const int off = s.nk - s.nq;
+  const bool split = a.groups > 0;                                     // the sinks' far queries are other workgroups' (far_keys)
+  // the queries that see key j: i = lo(j) .. hi(j)
+  auto lo = [&](int j) WIN_INLINE { return j - a.right - off; };
+  auto hi = [&](int j) WIN_INLINE { return !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
+  const int jend = min(j0 + 127, s.nk - 1);
+  const int i0 = max(0, lo(j0)), i1 = !split && j0 < a.sinks ? s.nq - 1 : hi(jend);
+  const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1, count = nt * G;
+  const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
+  const Stager<D> sq(a.ldq), sd(a.lddo);
+  auto stage = [&](int n) WIN_INLINE { stage_queries<D>(a, s, sq, sd, pl.h * G + n / nt, t0 + n % nt, l0 + (n & 1) * ST, wave); };
+  const int jw = j0 + wave * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1), jwe = min(jw + 31, s.nk - 1);
   const float c = a.scale * LOG2E;
   s16x8 kf[D / 16], vf[D / 16];
   load_cols<D>(kf, a.k + (long long)(s.k0 + jc) * a.ldk + pl.h * (D * 2));
   load_cols<D>(vf, a.v + (long long)(s.k0 + jc) * a.ldv + pl.h * (D * 2));
   const int ilo = lo(j), ihi = j < s.nk ? hi(j) : -1;
-  const bool sink_w = jwe < a.sinks;                                    // the wave's keys are sinks all
+  const bool sink_w = !split && jwe < a.sinks;                                    // the wave's keys are sinks all
   // queries wlo .. whi see a key of the wave, flo .. fhi see them all
-  const int wlo = lo(jw), whi = far || (!split && jw < a.sinks) ? s.nq - 1 : hi(jwe);
-  const int flo = lo(jwe), fhi = far ? (sink_w ? s.nq - 1 : -1) : !split && sink_w ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);
-  const bool do_k = !far || wave >= 2, do_v = !far || wave < 2;
+  const int wlo = lo(jw), whi = !split && jw < a.sinks ? s.nq - 1 : hi(jwe);
+  const int flo = lo(jwe), fhi = sink_w ? s.nq - 1 : min(s.nq - 1, jw + a.left - off);
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
-  if (na < nb) stage(na);
-  for (int n = na; n < nb; ++n) {
+  if (count) stage(0);
+  for (int n = 0; n < count; ++n) {
     tile_barrier();
-    if (n + 1 < nb) stage(n + 1);
+    if (n + 1 < count) stage(n + 1);
     const int it = (t0 + n % nt) * TILE;
     const char* Qt = lds + (n & 1) * ST;
     const char* Dt = Qt + TB;
@@ -397,16 +468,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int iu = it + u * 32;
-      if (jw >= s.nk || iu > whi || iu + 31 < wlo || (far && u != (wave & 1))) continue;
+      if (jw >= s.nk || iu > whi || iu + 31 < wlo) continue;
       f32x16 st, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[r] = dp[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) st = mfma32<T>(row_frag32<D>(Qt, u * 32, ks), kf[ks], st);
-      if (do_k) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
-      }
+      for (int ks = 0; ks < D / 16; ++ks) dp = mfma32<T>(row_frag32<D>(Dt, u * 32, ks), vf[ks], dp);
       if (iu < flo || iu + 31 > fhi) mask_queries(st, iu + 4 * half, ilo, ihi);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -419,37 +488,31 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
           dp[r] -= de[e];
         }
       }
-      if (do_v) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const s16x8 pf = pack8<T>(st, h);
+      for (int h = 0; h < 2; ++h) {
+        const s16x8 pf = pack8<T>(st, h);
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) dv[dt] = mfma32<T>(col_frag32<D>(Dt, u * 32 + h * 16, dt), pf, dv[dt]);
-        }
+        for (int dt = 0; dt < D / 32; ++dt) dv[dt] = mfma32<T>(col_frag32<D>(Dt, u * 32 + h * 16, dt), pf, dv[dt]);
       }
-      if (do_k) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] *= st[r];
+      for (int r = 0; r < 16; ++r) dp[r] *= st[r];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const s16x8 sf = pack8<T>(dp, h);
+      for (int h = 0; h < 2; ++h) {
+        const s16x8 sf = pack8<T>(dp, h);
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) dk[dt] = mfma32<T>(col_frag32<D>(Qt, u * 32 + h * 16, dt), sf, dk[dt]);
-        }
+        for (int dt = 0; dt < D / 32; ++dt) dk[dt] = mfma32<T>(col_frag32<D>(Qt, u * 32 + h * 16, dt), sf, dk[dt]);
       }
     }
   }
-  if (far || (split && jw < a.sinks)) {
-    // [slot][dK, dV][D][32 keys]; slots: (piece, half of its tiles), last the window's own
-    const int slots = 2 * a.pieces + 1, slot = far ? 2 * piece + (wave & 1) : slots - 1, gi = far ? group : jw / 32;
-    float* sl = a.slabs + (((size_t)(pl.b * a.Hkv + pl.h) * a.groups + gi) * slots + slot) * (2 * D * 32) + (lane & 31);
+  if (split && jw < a.sinks) {
+    float* sk = slab<D>(a, pl.b, pl.h, jw / 32, 2 * a.pieces, false) + (lane & 31);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int d = dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (do_k) sl[d * 32] = dk[dt][r];
-        if (do_v) sl[(D + d) * 32] = dv[dt][r];
+        sk[d * 32] = dk[dt][r];
+        sk[(D + d) * 32] = dv[dt][r];
       }
     return;
   }
@@ -472,10 +535,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void win_bwd_kv_kernel(WinArg
 // The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other
 // through the LDS, and then one adds up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum
 // instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above: 111 us = 497 TFLOP/s.
-template <class T, int D>
-__global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
+template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, char* lds) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * ST + 8192];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
   Place pl;
   if (!place(a, (a.max_k + 63) / 64, a.Hkv, pl)) return;
@@ -483,7 +544,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
   const int j0 = pl.tile * 64;
   if (j0 >= s.nk) return;
   const int off = s.nk - s.nq;
-  const bool split = a.groups > 0;                                     // the sinks' far queries are the other kernel's (far)
+  const bool split = a.groups > 0;                                     // the sinks' far queries are other workgroups' (far_keys)
   auto lo = [&](int j) WIN_INLINE { return j - a.right - off; };       // the queries that see key j
   auto hi = [&](int j) WIN_INLINE { return !split && j < a.sinks ? s.nq - 1 : min(s.nq - 1, j + a.left - off); };
   const int jend = min(j0 + 63, s.nk - 1);
@@ -491,18 +552,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
   const int t0 = i0 / TILE, nt = i1 < i0 ? 0 : i1 / TILE - t0 + 1, count = nt * G;
   const uint32_t l0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)lds);
   const Stager<D> sq(a.ldq), sd(a.lddo);
-  auto stage = [&](int g, int t, int buf) WIN_INLINE {
-    const int i0 = t * TILE, h = pl.h * G + g, last = s.nq - 1 - i0;
-    const long long row = s.q0 + i0;
-    const uint32_t l = l0 + buf * ST;
-    sq(a.q + row * a.ldq + h * (D * 2), last, l);
-    sd(a.dout + row * a.lddo + h * (D * 2), last, l + TB);
-    if (wave < 2) {
-      const float* src = (wave ? a.delta : a.lse2) + (size_t)h * a.rows_q + row;
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
-                   : : "v"((uint32_t)min(lane, last) * 4u), "s"(src), "s"(l + 2 * TB + wave * 256) : "memory", "m0");
-    }
-  };
+  auto stage = [&](int g, int t, int buf) WIN_INLINE { stage_queries<D>(a, s, sq, sd, pl.h * G + g, t, l0 + buf * ST, wave); };
   const int u = wave >> 1;                                             // the wave's half of a tile; 0 adds up dV, 1 dK
   const int jw = j0 + (wave & 1) * 32, j = jw + (lane & 31), jc = min(j, s.nk - 1), jwe = min(jw + 31, s.nk - 1);
   const float c = a.scale * LOG2E;
@@ -583,9 +633,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
     ++t1;
   }
   if (split && jw < a.sinks) {
-    // the window's own slot of the slabs
-    const int slots = 2 * a.pieces + 1;
-    float* sl = a.slabs + (((size_t)(pl.b * a.Hkv + pl.h) * a.groups + jw / 32) * slots + slots - 1) * (2 * D * 32) + (u ? 0 : D * 32) + (lane & 31);
+    float* sl = slab<D>(a, pl.b, pl.h, jw / 32, 2 * a.pieces, !u) + (lane & 31);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -605,6 +653,19 @@ __global__ __launch_bounds__(256, 2) void win_bwd_kv2_kernel(WinArgs a) {
       for (int e = 0; e < 4; ++e) x[e] = (T)(sum[dt][4 * g + e] * f);
       *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = x;
     }
+}
+
+// heads of 64: both sums of 32 keys fit a wave beside another wave's (two 16-frame clips 180 us, shared in pairs 194); heads of 128:
+// they do not (six packed texts 182 us, in pairs 138)
+constexpr int keys_of_a_workgroup(int D) { return D == 64 ? 128 : 64; }
+template <class T, int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void win_bwd_kv_kernel(WinArgs a) {
+  constexpr int ST = 2 * TILE * D * 2 + 512;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * ST + (D == 64 ? 0 : 8192)];
+  const int far = (int)blockIdx.x - (int)gridDim.x + a.far_blocks;
+  if (far >= 0) far_keys<T, D>(a, lds, far);
+  else if constexpr (D == 64) window_keys<T, D>(a, lds);
+  else window_keys_in_pairs<T, D>(a, lds);
 }
 
 // the sinks' slabs, added slot by slot (every eighth one a thread, then the eight): a workgroup = 32 keys, 8 values of dK or dV each
@@ -644,18 +705,18 @@ __global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
   *reinterpret_cast<T8*>(p + h * (D * 2) + (is_v ? d8 - D / 8 : d8) * 16) = y;
 }
 
-// how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries; 0 groups: the sinks' own tiles walk all
-// queries.  That takes max_q / 64 steps where a window's tile takes (left + right + 128) / 64: split where it is over 512 queries longer.
-// (Of many sinks - over 512 keys - the tiles themselves are enough workgroups, and the slabs would be large.)
+// how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries, each about half as many as a window's tile walks
+// (as many: packed texts 121 us instead of 115); 0 groups: the sinks' own tiles walk all queries.  That takes max_q / 64 steps where a window's tile takes (left + right + 128) / 64:
+// split where it is over 512 queries longer.  (Of many sinks - over 512 keys - the tiles themselves are enough workgroups, and the slabs
+// would be large.)
 struct FarSplit { int groups, pieces; };
 static FarSplit far_split(int B, int Hq, int Hkv, int D, int max_q, int max_k, int left, int sinks) {
   const long long rows = min((long long)max_q, (long long)max_k - left);
   if (sinks < 1 || min(sinks, max_k) > 512 || rows <= 512 || B < 1) return {0, 0};
   const int groups = (min(sinks, max_k) + 31) / 32;
-  if ((long long)B * Hkv * groups * (2 * D / 8) >= 1ll << 24) return {0, 0};              // (win_bwd_sink_kernel: a launch holds 2^32 threads)
-  // as many workgroups as stay resident: two a CU with heads of 64, one with heads of 128
-  const long long want = (D == 64 ? 512 : 256) / max(1ll, (long long)B * Hkv * groups);
-  return {groups, (int)max(1ll, min(want, rows * (Hq / Hkv) / 256))};
+  const long long pieces = min(256ll, 2 * rows / (left + 128) + 1);
+  if ((long long)B * Hkv * groups * max(pieces, 2ll * D / 8) >= 1ll << 23) return {0, 0};  // (a launch holds 2^32 threads)
+  return {groups, (int)pieces};
 }
 static size_t slab_floats(const FarSplit& f, int B, int Hkv, int D) {
   return (size_t)B * Hkv * f.groups * (2 * f.pieces + 1) * 2 * D * 32;
@@ -690,15 +751,8 @@ using namespace oat;
 
 #define WIN_FWD(T, D) win_fwd_kernel<T, D>
 #define WIN_Q(T, D) win_bwd_q_kernel<T, D>
-#define WIN_FAR(T, D) win_bwd_kv_kernel<T, D, true>
-#define WIN_KV(T, D) win_bwd_kv_kernel<T, D, false>
-#define WIN_KV2(T, D) win_bwd_kv2_kernel<T, D>
+#define WIN_KV(T, D) win_bwd_kv_kernel<T, D>
 #define WIN_SINK(T, D) win_bwd_sink_kernel<T, D>
-#define WIN_LAUNCH1(kernel, DD, grid)                                                                                \
-  do {                                                                                                               \
-    if (dtype == 0) OAT_LAUNCH((kernel(bf16, DD)), dim3(grid), dim3(256), 0, s, a);                                  \
-    else OAT_LAUNCH((kernel(_Float16, DD)), dim3(grid), dim3(256), 0, s, a);                                         \
-  } while (0)
 #define WIN_LAUNCH(kernel, grid) WIN_LAUNCH2(kernel, dim3(grid))
 #define WIN_LAUNCH2(kernel, grid)                                                                                    \
   do {                                                                                                               \
@@ -770,15 +824,11 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   a.groups = f.groups;
   a.pieces = f.pieces;
   a.slabs = a.delta + (size_t)rows_q * Hq;
-  if (max_k && rows_k && f.groups) WIN_LAUNCH(WIN_FAR, (long long)B * Hkv * f.groups * f.pieces);
   if (max_k && rows_k) {
-    // heads of 64: both sums of 32 keys fit a wave beside another wave's (two 16-frame clips 180 us, shared in pairs 194); heads of 128:
-    // they do not (six packed texts 182 us, in pairs 138)
-    const int tiles = D == 64 ? (max_k + 127) / 128 : (max_k + 63) / 64;
+    const int tiles = (max_k + keys_of_a_workgroup(D) - 1) / keys_of_a_workgroup(D);
     a.run = deal_run(B, Hkv, 1, tiles, rows_k, max_k);
-    const unsigned grid = deal_grid((long long)B * Hkv * tiles, a.run);
-    if (D == 64) WIN_LAUNCH1(WIN_KV, 64, grid);
-    else WIN_LAUNCH1(WIN_KV2, 128, grid);
+    a.far_blocks = B * Hkv * f.groups * f.pieces;
+    WIN_LAUNCH(WIN_KV, deal_grid((long long)B * Hkv * tiles, a.run) + a.far_blocks);
   }
   if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 8));
   return check_launch("attn_window_bwd");
