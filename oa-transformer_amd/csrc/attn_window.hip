@@ -83,6 +83,29 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
     P[1] = pack8<T>(E, 1);
     return t;
   };
+  auto begin = [&](const f32x16& S) WIN_INLINE {
+    const float mx = row_max(S);
+    if (!begun && mx > -INFINITY) {
+      neg = -mx * c;
+      begun = true;
+    }
+    all_begun = __all(begun);
+  };
+  auto settle = [&](const f32x16& S, s16x8 (&P)[2], float t) WIN_INLINE {
+    if (__any(t > 1024.f)) {
+      const float to = fminf(neg, -row_max(S) * c);                    // (a row that sees nothing here: +inf, the minimum stays)
+      float al = __builtin_amdgcn_exp2f(begun ? to - neg : 0.f);
+      if (begun) neg = to;
+      asm volatile("" : "+v"(al));                                     // (nothing of this before the branch)
+      l *= al;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= al;
+      t = exponentials(S, P);
+    }
+    l += t;
+  };
   // One step = 32 keys: their exponentials (vector unit) beside the products of the 32 before (values) and after (scores), which do not
   // depend on them.  The scheduling groups deal the products out over the exponentials: one unit would wait for the other otherwise.
   // The reference is the maximum of the first keys a row sees, not a running one (a third of the vector work): it moves only when a sum
@@ -97,16 +120,9 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) vf[h][dt] = col_frag32<D>(V, (1 - u) * 32 + h * 16, dt);
     const int j0 = kt.at(n) * TILE + u * 32;
-    const bool edge_hi = j0 + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = j0 < wp1 - a.left && j0 + 31 >= a.sinks;
-    if (edge_lo | edge_hi) mask_keys(S, j0 + 4 * half, lo, hi, a.sinks, edge_lo, edge_hi);
-    if (!all_begun) {
-      const float mx = row_max(S);
-      if (!begun && mx > -INFINITY) {
-        neg = -mx * c;
-        begun = true;
-      }
-      all_begun = __all(begun);
-    }
+    const bool edge_hi = j0 + 31 > min(s.nk - 1, wp0 + a.right), edge_lo = j0 < wp1 - a.left;
+    if (edge_lo | edge_hi) mask_keys(S, j0 + 4 * half, lo, hi, 0, edge_lo, edge_hi);
+    if (!all_begun) begin(S);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) Sq[r] = 0.f;
@@ -124,19 +140,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
       __builtin_amdgcn_sched_group_barrier(0x002, 64 / (D / 8), 0);    // vector instructions
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (__any(t > 1024.f)) {
-      const float to = fminf(neg, -row_max(S) * c);                    // (a row that sees nothing here: +inf, the minimum stays)
-      float al = __builtin_amdgcn_exp2f(begun ? to - neg : 0.f);
-      if (begun) neg = to;
-      asm volatile("" : "+v"(al));                                     // (nothing of this before the branch)
-      l *= al;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= al;
-      t = exponentials(S, P);
-    }
-    l += t;
+    settle(S, P, t);
   };
   // K of tiles n, n + 1 and V of tiles n - 1, n are in use at tile n, so the next copies start between its two steps
   P1[0] = P1[1] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -159,13 +163,32 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
     turn(n, odd);
     step(n, 1, S1, P1, V1, P0, K1, S0);
   };
-  // the wave's own tiles na .. nb - 1 of the list (those between that only other waves see are masked).  The loop has no branch around
-  // the sums - where paths with and without products meet, the compiler copies all of o - and two tiles a turn, so that all LDS
-  // addresses are constants.
-  const int hw = iw < s.nq ? min(s.nk - 1, wp1 + a.right) : -1, ht = hw / TILE;
-  const int nb = hw < 0 ? 0 : ht < kt.sink ? ht + 1 : max(kt.sink, ht - kt.first + kt.sink + 1);
-  const int na = kt.sink ? 0 : min(nb, max(0, max(0, wp0 - a.left) / TILE - kt.first));
+  // The sinks' tiles, one after the other: often a few keys, of which a wave looks at the halves it sees.  (In the loop below, with
+  // tiles between them and the window masked: 8191 tokens with four sinks 184 us instead of 180, others equal.)
+  const int hw = iw < s.nq ? min(s.nk - 1, wp1 + a.right) : -1;
+  auto seen = [&](int j0) WIN_INLINE { return j0 <= hw && (j0 < a.sinks || j0 + 31 >= wp0 - a.left); };
+  auto alone = [&](f32x16& S, int j0, const char* V, int u) WIN_INLINE {
+    mask_keys(S, j0 + 4 * half, lo, hi, a.sinks, true, true);
+    if (!all_begun) begin(S);
+    s16x8 P[2];
+    const float t = exponentials(S, P);
+    settle(S, P, t);
+    values(V, u, P);
+  };
   int n = 0;
+  for (; n < kt.sink; ++n) {
+    const int j0 = n * TILE, odd = n & 1;
+    const bool seen0 = seen(j0), seen1 = seen(j0 + 32);
+    if (seen0) scores(lds + odd * TB, 0, S0);
+    if (seen1) scores(lds + odd * TB, 1, S1);
+    turn(n, odd);
+    if (seen0) alone(S0, j0, lds + (2 + odd) * TB, 0);
+    if (seen1) alone(S1, j0 + 32, lds + (2 + odd) * TB, 1);
+  }
+  // the wave's own tiles of the window, na .. nb - 1 of the list.  The loop has no branch around the sums - where paths with and without
+  // products meet, the compiler copies all of o - and two tiles a turn, so that all LDS addresses are constants.
+  const int nb = hw < 0 ? 0 : hw / TILE - kt.first + kt.sink + 1;
+  const int na = min(nb, kt.sink + max(0, max(0, wp0 - a.left) / TILE - kt.first));
   for (; n < na; ++n) turn(n, n & 1);
   if (n < nb) {
     scores(lds + (n & 1) * TB, 0, S0);
