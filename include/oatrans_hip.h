@@ -331,13 +331,14 @@ int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long
                           void* k_cache, void* v_cache, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream);
 
 /* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
- * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused), attention with the sequences' query rows as their key rows, out [M, Hq * D]
- * dense, and - with k_cache - the prompt's cache.  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back; workspace as for
+ * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused; table, if not NULL: the cos and sin of every row's pairs, fp32 [n_pairs, M, 2]), attention with the sequences' query rows as their key rows, out [M, Hq * D]
+ * dense, and - with k_cache - the prompt's cache.  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back (with the forward's table, of
+ * pairs that are a head's two halves, before its rounding; else in a pass of its own); workspace as for
  * oat_attn_window_bwd with max_q = max_k = longest. */
-int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, const OatRope* rope, const int* pos, int period, void* out, float* lse,
+int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out, float* lse,
                              const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks,
                              float scale, void* k_cache, void* v_cache, const long long* strides, int cap, void* stream);
-int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const OatRope* rope, const int* pos, int period, const void* out,
+int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period, const void* out,
                              const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D,
                              int dtype, int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -34,21 +34,24 @@ def rope_axes(x, pos, rope, heads, head_dim):
 
 
 def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, cache):
-    """-> (out, turned q | k or None): rotary positions into a new buffer (the values stay where they are), attention over it, and the
-    prompt's rows into the cache, in one call."""
+    """-> (out, turned q | k or None, the turns or None): rotary positions into a new buffer (the values stay where they are), attention
+    over it, and the prompt's rows into the cache, in one call.  The turns - every row's cos and sin - are kept for a backward pass
+    that can use them (pairs that are a head's two halves)."""
     M, dev, dt = qkv.shape[0], qkv.device, qkv.dtype
     what = "window_attention"
     if qkv.stride(1) != 1 or (dt is not torch.bfloat16 and dt is not torch.float16):
         raise hip.OatError(f"{what}: qkv must be bf16 or fp16 with unit column stride")
     if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous() or seqs.device != dev:
         raise hip.OatError(f"{what}: seqs must be a contiguous int32 [B, 4] on {dev}")
-    qk = turned = struct = places = None
+    qk = turned = turns = struct = places = None
     period = 0
     if rope is not None:
         if pos.dtype is not torch.int32 or pos.dim() != 2 or pos.shape[1] != rope.axes or not pos.is_contiguous() or pos.device != dev:
             raise hip.OatError(f"{what}: pos must be a contiguous int32 [P, {rope.axes}] on {dev}")
         qk = torch.empty(M, (heads + kv_heads) * D, dtype=dt, device=dev)
         turned, struct, places, period = qk.data_ptr(), rope.struct, pos.data_ptr(), pos.shape[0]
+        if lse is not None and 2 * rope.pairs == D and not rope.interleaved:
+            turns = torch.empty(rope.pairs, M, 2, dtype=torch.float32, device=dev)
     out = (torch.empty if packed else torch.zeros)(M, heads * D, dtype=dt, device=dev)
     kc = vc = strides = None
     cap = 0
@@ -59,28 +62,28 @@ def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, p
             raise hip.OatError(f"{what}: the caches must be [{seqs.shape[0]}, slots, {kv_heads}, {D}] of {dt} on {dev}")
         kc, vc = k.data_ptr(), v.data_ptr()
     hip._launch(dev, hip.lib().oat_window_attention_fwd, (
-        qkv.data_ptr(), hip._ld(qkv), turned, struct, places, period, out.data_ptr(), lse.data_ptr() if lse is not None else None,
+        qkv.data_ptr(), hip._ld(qkv), turned, turns.data_ptr() if turns is not None else None, struct, places, period, out.data_ptr(), lse.data_ptr() if lse is not None else None,
         seqs.data_ptr(), seqs.shape[0], longest, M, heads, kv_heads, D, hip._ELEMENTS[dt], *window, D ** -0.5 if scale is None else scale,
         kc, vc, strides, cap), what)
-    return out, qk
+    return out, qk, turns
 
 
 class _WindowFn(torch.autograd.Function):
     """Rotary positions, attention over the window and its sinks, and the gradient of all of it with respect to qkv.  Saved: qkv, the
-    turned q | k, out and the log-sum-exp; backward forms the probabilities again."""
+    turned q | k, the turns, out and the log-sum-exp; backward forms the probabilities again."""
 
     @staticmethod
     def forward(ctx, qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed):
         lse = torch.empty(qkv.shape[0], heads, dtype=torch.float32, device=qkv.device)
-        out, qk = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, None)
-        ctx.save_for_backward(qkv, qk, out, lse, seqs, pos)
+        out, qk, turns = _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, None)
+        ctx.save_for_backward(qkv, qk, turns, out, lse, seqs, pos)
         ctx.args = heads, kv_heads, D, longest, window, scale, rope, packed
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, qk, out, lse, seqs, pos = ctx.saved_tensors
+        qkv, qk, turns, out, lse, seqs, pos = ctx.saved_tensors
         heads, kv_heads, D, longest, window, scale, rope, packed = ctx.args
         dout, dev, lib = dout.contiguous(), qkv.device, hip.lib()
         if dout.data_ptr() % 16:
@@ -90,7 +93,8 @@ class _WindowFn(torch.autograd.Function):
         need = lib.oat_attn_window_bwd_workspace_bytes(M, B, longest, longest, heads, kv_heads, D, window[0], window[2])
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         hip._launch(dev, lib.oat_window_attention_bwd, (
-            qkv.data_ptr(), hip._ld(qkv), qk.data_ptr() if qk is not None else None, rope.struct if rope is not None else None,
+            qkv.data_ptr(), hip._ld(qkv), qk.data_ptr() if qk is not None else None,
+            turns.data_ptr() if turns is not None else None, rope.struct if rope is not None else None,
             pos.data_ptr() if pos is not None else None, pos.shape[0] if pos is not None else 0, out.data_ptr(), lse.data_ptr(),
             dout.data_ptr(), dqkv.data_ptr(), seqs.data_ptr(), B, longest, M, heads, kv_heads, D, hip._ELEMENTS[qkv.dtype], *window,
             D ** -0.5 if scale is None else scale, ws.data_ptr(), need), "window_attention backward")

@@ -44,8 +44,8 @@ _WINDOW_SIGNATURES = {
     "oat_attn_window_bwd": (_I, [_P, _L] * 4 + [_P] + [_P, _L] * 4 + [_P] + [_I] * 12 + [_F, _P, _Z, _P]),
     "oat_attn_window_step_workspace_bytes": (_Z, [_I] * 4),
     "oat_attn_window_step": (_I, [_P, _L, _P, _P, _P, ctypes.POINTER(_L), _I, _P, _L] + [_I] * 8 + [_F, ctypes.POINTER(_OatRope), _P, _P, _Z, _P]),
-    "oat_window_attention_fwd": (_I, [_P, _L, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P] + [_I] * 10 + [_F, _P, _P, ctypes.POINTER(_L), _I, _P]),
-    "oat_window_attention_bwd": (_I, [_P, _L, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P, _P, _P] + [_I] * 10 + [_F, _P, _Z, _P]),
+    "oat_window_attention_fwd": (_I, [_P, _L, _P, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P] + [_I] * 10 + [_F, _P, _P, ctypes.POINTER(_L), _I, _P]),
+    "oat_window_attention_bwd": (_I, [_P, _L, _P, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P, _P, _P] + [_I] * 10 + [_F, _P, _Z, _P]),
     "oat_window_cache_fill": (_I, [_P, _L, _P, _L, _P, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _I, _I, _I, _P]),
 }
 

@@ -96,6 +96,21 @@ template <int D> OAT_DEV void load_cols(s16x8 (&f)[D / 16], const char* row) {
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) f[ks] = *reinterpret_cast<const s16x8*>(row + (2 * ks + half) * 16);
 }
+// turns the sums of a row (C fragments of the transposed product: a lane holds half of one row) back by its pairs' cos and sin.  A pair is
+// (d, d + D / 2): one register of two fragments.  `turns` points to the row's first pair, `pitch` rows a pair: the lanes read neighbouring
+// rows (with the pairs of a row side by side a wave's read touched 64 lines: six packed texts' query gradients 80 -> 91 us; so: 87).
+template <int D> OAT_DEV void turn_back(f32x16 (&x)[D / 32], const float2* turns, int pitch) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int dt = 0; dt < D / 64; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float2 w = turns[(size_t)(dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3)) * pitch];
+      const float2 y = rope_turn(x[dt][r], x[dt + D / 64][r], float2{w.x, -w.y});
+      x[dt][r] = y.x;
+      x[dt + D / 64][r] = y.y;
+    }
+}
 // maximum / sum of a value over lanes l and l ^ 32 (one register swap of the halves, no LDS)
 OAT_DEV float both_halves(float v, bool max) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
@@ -126,6 +141,7 @@ struct WinArgs {
   int run;                              // tiles that go to one XCD together
   int groups, pieces, far_blocks;       // how the sinks' far queries are split; their workgroups in the launch
   float scale;
+  const float2* turns;                  // backward: cos and sin of [D / 2, rows_q] pairs (p, p + D / 2) to turn dq and dk back by, or null
 };
 struct Seq { int q0, nq, k0, nk; };
 // a sequence that does not fit the buffers (or the launch) is taken as empty: nothing outside is read or written
@@ -208,5 +224,11 @@ OAT_DEV KeyTiles key_tiles(const WinArgs& a, int nk, int p0, int p1) {
   const int first = max(max(0, p0 - a.left) / TILE, sink);
   return {sink, first, sink + max(0, end - first)};
 }
+
+// oat_attn_window_bwd; `turns` (may be null): dq and dk are turned back by these before they are rounded (WinArgs::turns; rows_q = rows_k)
+int attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out, long long ldo,
+                    const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk, long long lddk, void* dv,
+                    long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
+                    int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, const float2* turns, void* stream);
 
 }  // namespace oat

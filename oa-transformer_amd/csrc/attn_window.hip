@@ -231,7 +231,8 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
 // summed in the workgroup): 7 products for the 5 of one kernel with atomic sums, but every sum has one fixed order.
 
 // dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  Bound: instruction issue, as above, with three products
-// for one exponential: the clips of above 139 us = 775 TFLOP/s, the packed texts 80 us = 517.
+// for one exponential: the clips of above 139 us = 775 TFLOP/s, the packed texts 80 us = 517 (141 and 87 with the
+// turn back).
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
@@ -328,6 +329,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   }
   if (n < kt.count) tile(n, 0);
   if (i >= s.nq) return;
+  if (a.turns) turn_back<D>(dq, a.turns + row, a.rows_q);
   char* po = a.dq + row * a.lddq + pl.h * (D * 2);
   typedef __attribute__((ext_vector_type(4))) T T4;
 #pragma unroll
@@ -540,6 +542,7 @@ template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) 
     return;
   }
   if (j >= s.nk) return;
+  if (a.turns) turn_back<D>(dk, a.turns + s.k0 + j, a.rows_q);
   char* pk = a.dk + (long long)(s.k0 + j) * a.lddk + pl.h * (D * 2);
   char* pv = a.dv + (long long)(s.k0 + j) * a.lddv + pl.h * (D * 2);
   typedef __attribute__((ext_vector_type(4))) T T4;
@@ -557,7 +560,8 @@ template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) 
 
 // The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other
 // through the LDS, and then one adds up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum
-// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above: 111 us = 497 TFLOP/s.
+// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above: 111 us = 497 TFLOP/s
+// (115 with the sinks' far queries, 121 with the turn back too).
 template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, char* lds) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
@@ -664,6 +668,7 @@ template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, ch
     return;
   }
   if (j >= s.nk) return;
+  if (u && a.turns) turn_back<D>(sum, a.turns + s.k0 + j, a.rows_q);
   const float f = u ? a.scale : 1.f;
   char* po = (u ? a.dk + (long long)(s.k0 + j) * a.lddk : a.dv + (long long)(s.k0 + j) * a.lddv) + pl.h * (D * 2);
   typedef __attribute__((ext_vector_type(4))) T T4;
@@ -691,41 +696,56 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void win_bwd_kv_kernel(WinArg
   else window_keys_in_pairs<T, D>(a, lds);
 }
 
-// the sinks' slabs, added slot by slot (every eighth one a thread, then the eight): a workgroup = 32 keys, 8 values of dK or dV each
+// the sinks' slabs, added slot by slot (every eighth one a thread, then the eight): a workgroup = 32 keys, two chunks of 8 values of dK or
+// dV half a head apart, which are pairs of the rotary positions
 template <class T, int D>
 __global__ __launch_bounds__(256) void win_bwd_sink_kernel(WinArgs a) {
-  __shared__ float part[8][8][32];
-  const int key = threadIdx.x & 31, w = threadIdx.x >> 5, d8 = blockIdx.y;              // d8: 0 .. 2 D / 8
+  __shared__ float part[8][16][32];
+  const int key = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const bool is_v = blockIdx.y >= D / 16;
+  const int d8 = blockIdx.y % (D / 16) * 8;
   const int group = blockIdx.x % a.groups, h = blockIdx.x / a.groups % a.Hkv, b = blockIdx.x / a.groups / a.Hkv;
   const Seq s = load_seq(a, b);
   if (group * 32 >= min(a.sinks, s.nk)) return;
   const int slots = 2 * a.pieces + 1;
-  const float* sl = a.slabs + ((size_t)blockIdx.x * slots + w) * (2 * D * 32) + d8 * 8 * 32 + key;
-  float x[8];
+  const float* sl = slab<D>(a, b, h, group, w, is_v) + d8 * 32 + key;
+  float x[16];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-#pragma unroll 4
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+#pragma unroll 2
   for (int i = w; i < slots; i += 8, sl += 8 * 2 * D * 32) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] += sl[e * 32];
+    for (int e = 0; e < 16; ++e) x[e] += sl[(e < 8 ? e : e - 8 + D / 2) * 32];
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[w][e][key] = x[e];
+  for (int e = 0; e < 16; ++e) part[w][e][key] = x[e];
   __syncthreads();
   const int j = group * 32 + key;
   if (w || j >= s.nk) return;
-  const bool is_v = d8 >= D / 8;
-  typedef __attribute__((ext_vector_type(8))) T T8;
-  T8 y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float v = part[0][e][key];
+  for (int e = 0; e < 16; ++e) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) v += part[k][e][key];
-    y[e] = (T)(is_v ? v : v * a.scale);
+    for (int k = 1; k < 8; ++k) x[e] += part[k][e][key];
   }
-  char* p = is_v ? a.dv + (long long)(s.k0 + j) * a.lddv : a.dk + (long long)(s.k0 + j) * a.lddk;
-  *reinterpret_cast<T8*>(p + h * (D * 2) + (is_v ? d8 - D / 8 : d8) * 16) = y;
+  const long long row = s.k0 + j;
+  if (!is_v && a.turns) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 t = a.turns[(size_t)(d8 + e) * a.rows_q + row], y = rope_turn(x[e], x[8 + e], float2{t.x, -t.y});
+      x[e] = y.x;
+      x[8 + e] = y.y;
+    }
+  }
+  typedef __attribute__((ext_vector_type(8))) T T8;
+  char* p = (is_v ? a.dv + row * a.lddv : a.dk + row * a.lddk) + h * (D * 2);
+  const float f = is_v ? 1.f : a.scale;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    T8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (T)(x[8 * c + e] * f);
+    *reinterpret_cast<T8*>(p + (d8 + c * (D / 2)) * 2) = y;
+  }
 }
 
 // how the far pairs of the sinks are split: groups of 32 sink keys, pieces of their queries, each about half as many as a window's tile walks
@@ -738,7 +758,7 @@ static FarSplit far_split(int B, int Hq, int Hkv, int D, int max_q, int max_k, i
   if (sinks < 1 || min(sinks, max_k) > 512 || rows <= 512 || B < 1) return {0, 0};
   const int groups = (min(sinks, max_k) + 31) / 32;
   const long long pieces = min(256ll, 2 * rows / (left + 128) + 1);
-  if ((long long)B * Hkv * groups * max(pieces, 2ll * D / 8) >= 1ll << 23) return {0, 0};  // (a launch holds 2^32 threads)
+  if ((long long)B * Hkv * groups * max(pieces, (long long)D / 8) >= 1ll << 23) return {0, 0};  // (a launch holds 2^32 threads)
   return {groups, (int)pieces};
 }
 static size_t slab_floats(const FarSplit& f, int B, int Hkv, int D) {
@@ -813,11 +833,11 @@ extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max
   return ((size_t)rows_q * Hq * 2 + slab_floats(far_split(B, Hq, Hkv, D, max_q, max_k, far(left), sinks), B, Hkv, D)) * 4;
 }
 
-extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
-                                   long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
-                                   long long lddk, void* dv, long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q,
-                                   int rows_k, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+int oat::attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
+                         long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
+                         long long lddk, void* dv, long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k,
+                         int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
+                         size_t workspace_bytes, const float2* turns, void* stream) {
   if (int rc = window_wrong("attn_window_bwd", seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, sinks, scale)) return rc;
   if (B == 0) return 0;
   if (rows_q && (rows_wrong(q, ldq, Hq, D) || rows_wrong(out, ldo, Hq, D) || rows_wrong(dout, lddo, Hq, D) || rows_wrong(dq, lddq, Hq, D) || !lse)) {
@@ -837,6 +857,7 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
   a.seqs = (const int4*)seqs;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
   a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
+  a.turns = turns;
   hipStream_t s = (hipStream_t)stream;
   if (max_q && rows_q) {
     const int tiles = (max_q + 127) / 128;
@@ -853,6 +874,15 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
     a.far_blocks = B * Hkv * f.groups * f.pieces;
     WIN_LAUNCH(WIN_KV, deal_grid((long long)B * Hkv * tiles, a.run) + a.far_blocks);
   }
-  if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, 2 * D / 8));
+  if (max_k && rows_k && f.groups) WIN_LAUNCH2(WIN_SINK, dim3(B * Hkv * f.groups, D / 8));
   return check_launch("attn_window_bwd");
+}
+
+extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out,
+                                   long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
+                                   long long lddk, void* dv, long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q,
+                                   int rows_k, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  return attn_window_bwd(q, ldq, k, ldk, v, ldv, out, ldo, lse, dout, lddo, dq, lddq, dk, lddk, dv, lddv, seqs, B, max_q, max_k, rows_q, rows_k,
+                         Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes, nullptr, stream);
 }

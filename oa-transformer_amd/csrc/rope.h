@@ -15,6 +15,11 @@ OAT_DEV float2 rope_cos_sin(int pos, double turns, bool inverse) {
   return float2{c, inverse ? -s : s};
 }
 
+// one pair turned; products and sums are spelt out, so that every kernel rounds alike
+OAT_DEV float2 rope_turn(float u, float v, float2 k) {
+  return float2{__builtin_fmaf(u, k.x, -(v * k.y)), __builtin_fmaf(v, k.x, u * k.y)};
+}
+
 // nullptr, or why a ladder cannot be used for heads of `dim` values
 inline const char* rope_wrong(const OatRope* r, int dim) {
   if (r->n_pairs < 1 || r->n_pairs > 64 || 2 * r->n_pairs > dim) return "the ladder has no pair, or more than the head (at most 64)";
@@ -25,6 +30,10 @@ inline const char* rope_wrong(const OatRope* r, int dim) {
   }
   return nullptr;
 }
+
+// oat_rope_axes; `table` (may be null): the cos and sin of every row's pairs, [n_pairs, M]
+int rope_axes(const void* x, long long ldx, void* out, long long ldo, int dtype, const int* pos, int period, int M, int heads, int dim,
+              const OatRope* rope, int inverse, float2* table, void* stream);
 
 // a 16-bit or 32-bit element type: vector loads, conversion
 template <class T> struct Elem;

@@ -17,6 +17,7 @@ struct RopeArgs {
   T* out; long long ldo;
   const int* pos; int period;                        // [period, n_axes]
   int M, heads, dim, rows, inverse;
+  float2* table;
   OatRope rope;
 };
 
@@ -41,7 +42,9 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
   for (int t = threadIdx.x; t < nr * np; t += 256) {
     const int r = t / np, p = t - r * np;
     const int pr = (m0 + r) % a.period;
-    cs[t] = rope_cos_sin(a.pos[(size_t)pr * a.rope.n_axes + a.rope.axis[p]], a.rope.turns[p], a.inverse != 0);
+    const float2 v = rope_cos_sin(a.pos[(size_t)pr * a.rope.n_axes + a.rope.axis[p]], a.rope.turns[p], a.inverse != 0);
+    cs[t] = v;
+    if (a.table) a.table[(size_t)p * a.M + m0 + r] = v;
   }
   __syncthreads();
   const bool copy = a.out != a.x;
@@ -60,20 +63,18 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
         V x = *reinterpret_cast<const V*>(px + c * N);
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) {
-          const float2 k = w[c * (N / 2) + e];
-          const float u = (float)x[2 * e], v = (float)x[2 * e + 1];
-          x[2 * e] = (T)(u * k.x - v * k.y);
-          x[2 * e + 1] = (T)(v * k.x + u * k.y);
+          const float2 y = rope_turn((float)x[2 * e], (float)x[2 * e + 1], w[c * (N / 2) + e]);
+          x[2 * e] = (T)y.x;
+          x[2 * e + 1] = (T)y.y;
         }
         store<FAR>(po + c * N, x);
       } else {
         V xu = *reinterpret_cast<const V*>(px + c * N), xv = *reinterpret_cast<const V*>(px + np + c * N);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float2 k = w[c * N + e];
-          const float u = (float)xu[e], v = (float)xv[e];
-          xu[e] = (T)(u * k.x - v * k.y);
-          xv[e] = (T)(v * k.x + u * k.y);
+          const float2 y = rope_turn((float)xu[e], (float)xv[e], w[c * N + e]);
+          xu[e] = (T)y.x;
+          xv[e] = (T)y.y;
         }
         store<FAR>(po + c * N, xu);
         store<FAR>(po + np + c * N, xv);
@@ -89,11 +90,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
       if (c >= np) {
         po[R + c - np] = px[R + c - np];
       } else {
-        const float2 k = cs[r * np + c];
         const int iu = a.rope.interleaved ? 2 * c : c, iv = a.rope.interleaved ? 2 * c + 1 : c + np;
-        const float u = (float)px[iu], v = (float)px[iv];
-        po[iu] = (T)(u * k.x - v * k.y);
-        po[iv] = (T)(v * k.x + u * k.y);
+        const float2 y = rope_turn((float)px[iu], (float)px[iv], cs[r * np + c]);
+        po[iu] = (T)y.x;
+        po[iv] = (T)y.y;
       }
     }
   }
@@ -101,8 +101,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
 
 template <class T>
 static int rope_run(const void* x, long long ldx, void* out, long long ldo, const int* pos, int period, int M, int heads, int dim,
-                    const OatRope* rope, int inverse, hipStream_t s) {
-  RopeArgs<T> a{(const T*)x, ldx, (T*)out, ldo, pos, period, M, heads, dim, 0, inverse, *rope};
+                    const OatRope* rope, int inverse, float2* table, hipStream_t s) {
+  RopeArgs<T> a{(const T*)x, ldx, (T*)out, ldo, pos, period, M, heads, dim, 0, inverse, table, *rope};
   constexpr int N = Elem<T>::N;
   const int np = rope->n_pairs;
   // about one angle per thread, but no fewer workgroups than four per CU while rows last
@@ -119,12 +119,8 @@ static int rope_run(const void* x, long long ldx, void* out, long long ldo, cons
   return check_launch("rope_axes");
 }
 
-}  // namespace oat
-
-using namespace oat;
-
-extern "C" int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dtype, const int* pos, int period, int M,
-                             int heads, int dim, const OatRope* rope, int inverse, void* stream) {
+int rope_axes(const void* x, long long ldx, void* out, long long ldo, int dtype, const int* pos, int period, int M, int heads, int dim,
+              const OatRope* rope, int inverse, float2* table, void* stream) {
   if (M < 0 || heads < 1 || dim < 2) { set_error("rope_axes: no heads, or a head of fewer than two values"); return -1; }
   if (M == 0) return 0;
   if (!x || !out || !pos || !rope) { set_error("rope_axes: x, out, pos and the ladder are needed"); return -1; }
@@ -135,10 +131,17 @@ extern "C" int oat_rope_axes(const void* x, long long ldx, void* out, long long 
   if (x == out && ldx != ldo) { set_error("rope_axes: in place needs one row pitch"); return -2; }
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case 0: return rope_run<bf16>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, s);
-    case 1: return rope_run<_Float16>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, s);
-    case 2: return rope_run<float>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, s);
+    case 0: return rope_run<bf16>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, table, s);
+    case 1: return rope_run<_Float16>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, table, s);
+    case 2: return rope_run<float>(x, ldx, out, ldo, pos, period, M, heads, dim, rope, inverse, table, s);
   }
   set_error("rope_axes: unknown element type");
   return -2;
+}
+
+}  // namespace oat
+
+extern "C" int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dtype, const int* pos, int period, int M,
+                             int heads, int dim, const OatRope* rope, int inverse, void* stream) {
+  return oat::rope_axes(x, ldx, out, ldo, dtype, pos, period, M, heads, dim, rope, inverse, nullptr, stream);
 }

@@ -175,7 +175,7 @@ def test_oracle_of_the_window_against_dense_attention():
     assert torch.allclose(wo.rope(y, pos, (4, 4), 50.0, inverse=True), x) and torch.allclose(y[1], x[1]) and torch.allclose(y.norm(dim=-1), x.norm(dim=-1))
 
 
-LAYER = dict(qkv=4096, ld=256, turned=None, rope=None, pos=None, period=0, out=4096, lse=None, seqs=4096, B=1, longest=10, M=10, Hq=2, Hkv=1, D=64,
+LAYER = dict(qkv=4096, ld=256, turned=None, table=None, rope=None, pos=None, period=0, out=4096, lse=None, seqs=4096, B=1, longest=10, M=10, Hq=2, Hkv=1, D=64,
              dtype=0, left=-1, right=0, sinks=0, scale=0.125, kc=None, vc=None, strides=None, cap=0)
 
 
@@ -192,7 +192,7 @@ def test_layer_refusals(change, text):
     _refused(hip, hip.lib().oat_window_attention_fwd(*a.values(), None), text)
     if "period" in change and text != b"turned":                   # (the way back turns last: its rotary arguments are the forward's)
         return
-    head = [a[n] for n in ("qkv", "ld", "turned", "rope", "pos", "period", "out")] + [4096, 4096, 4096]
+    head = [a[n] for n in ("qkv", "ld", "turned", "table", "rope", "pos", "period", "out")] + [4096, 4096, 4096]
     tail = [a[n] for n in ("seqs", "B", "longest", "M", "Hq", "Hkv", "D", "dtype", "left", "right", "sinks", "scale")]
     _refused(hip, hip.lib().oat_window_attention_bwd(*head, *tail, 4096, 1 << 40, None), text)
 
@@ -209,3 +209,11 @@ def test_workspaces_belong_to_their_sizes():
         with pytest.raises(hip.OatError, match="largest counts"):
             hip.attn_window_fwd(q, q, q, hip.seq_table([4], device="cpu"), 1, 1, 64, most, 4)
     assert [hip._reach(n) for n in (-7, -1, 0, 9, 2 ** 29, 2 ** 29 + 1, 2 ** 32, 2 ** 63)] == [-1, -1, 0, 9] + [2 ** 29] * 4
+
+
+def test_layer_backward_refuses_a_misaligned_table():
+    hip = _hip()
+    rope = hip.RopeAxes((64,)).struct
+    args = [4096, 256, 4096, 4100, rope, 4096, 10, 4096, 4096, 4096, 4096] + [LAYER[n] for n in (
+        "seqs", "B", "longest", "M", "Hq", "Hkv", "D", "dtype", "left", "right", "sinks", "scale")]
+    _refused(hip, hip.lib().oat_window_attention_bwd(*args, 4096, 1 << 40, None), b"not aligned")

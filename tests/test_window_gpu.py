@@ -269,6 +269,41 @@ def test_window_attention_gradient_with_rope(padded):
         assert (out[90 + 33:] == 0).all() and (g[90 + 33:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens,Hq,Hkv,D,sections,inter,left,right,sinks,gap", [
+    ([90, 33], 4, 2, 64, (16, 24, 24), False, 30, 10, 1, 5), ([1300, 700], 4, 1, 128, (128,), False, 100, 0, 40, 0),
+    ([2300], 1, 1, 64, (32, 32), False, 90, 3, 130, 0), ([1500, 1], 2, 2, 128, (32, 48, 48), False, 60, 60, 1, 2), ([70], 2, 1, 64, (48,), False, -1, -1, 0, 0),
+    ([70], 2, 1, 64, (64,), True, -1, 0, 3, 1), ([0, 17], 3, 3, 128, (128,), False, -1, 0, 0, 0)])
+def test_gradient_turned_back_where_it_is_formed(lens, Hq, Hkv, D, sections, inter, left, right, sinks, gap, dtype):
+    """The layer's dq and dk against those of the single operators turned back in 64 bits.  Both have the same 32-bit sums; the operators'
+    are rounded before the turn (each of a pair by half a step of its size), the layer's after it."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    M, n, L = sum(lens) + gap * len(lens), (Hq + Hkv) * D, max(lens)
+    starts = [sum(lens[:b]) + gap * (b + 1) for b in range(len(lens))]
+    table, rope = hip.seq_table(lens, q_rows=starts), hip.RopeAxes(sections, interleaved=inter)
+    qkv = rnd(M, n + Hkv * D, dtype=dtype, seed=11).requires_grad_()
+    pos = torch.randint(-40, 4000, (M, len(sections)), dtype=torch.int32, generator=torch.Generator().manual_seed(6)).to(DEV)
+    dout = rnd(M, Hq * D, dtype=dtype, seed=12)
+    out = wa.window_attention(qkv, table, Hq, Hkv, D, left, right, sinks, longest=L, rope=rope, pos=pos)
+    (g,) = torch.autograd.grad(out, qkv, dout)
+    x = qkv.detach()
+    qk, lse = hip.rope_axes(x[:, :n], pos, rope, Hq + Hkv, D), torch.zeros(M, Hq, device=DEV)
+    q, k, v = qk[:, :Hq * D], qk[:, Hq * D:], x[:, n:]
+    same = hip.attn_window_fwd(q, k, v, table, Hq, Hkv, D, L, L, left, right, sinks, lse=lse)
+    assert torch.equal(out, same)
+    dq, dk, dv = hip.attn_window_bwd(q, k, v, same, lse, dout, table, Hq, Hkv, D, L, L, left, right, sinks)
+    assert torch.equal(g[:, n:], dv)
+    d = torch.cat([dq, dk], 1).view(M, Hq + Hkv, D)
+    back = wo.rope(d, pos, sections, 10000.0, False, inter, inverse=True).view(M, n)
+    R = 2 * rope.pairs
+    a = d.double().abs()
+    other = a.clone()
+    other[..., :R] = a[..., :R].unflatten(-1, (-1, 2)).flip(-1).flatten(-2) if inter else a[..., :R].unflatten(-1, (2, -1)).flip(-2).flatten(-2)
+    u = half_step(dtype)
+    within(g[:, :n], back, (1.01 * u * (a + other)).view(M, n) + 1.01 * u * back.abs() + 4 * torch.finfo(dtype).tiny, "dq | dk")
+
+
 def test_window_attention_gradient_by_differences():
     """The directional derivative of the layer against central differences of the 64-bit definition."""
     hip = _hip()
