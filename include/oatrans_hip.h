@@ -326,9 +326,12 @@ size_t oat_attn_window_step_workspace_bytes(int B, int Hq, int Hkv, int D);
 int oat_attn_window_step(const void* qkv, long long ldqkv, const int* past, void* k_cache, void* v_cache, const long long* strides, int cap,
                          void* out, long long ldo, int B, int Hq, int Hkv, int D, int dtype, int left, int sinks, int rolling, float scale,
                          const OatRope* rope, const int* pos, void* workspace, size_t workspace_bytes, void* stream);
-/* A prompt's (turned) keys and values into a cache: slots as above; a prompt of more than cap tokens leaves its sinks and its last ones. */
+/* A prompt's (turned) keys and values into a cache: slots as above; a prompt of more than cap tokens leaves its sinks and its last ones.
+ * Keys that do not fit rows_k or max_k leave the cache as it was (in oat_window_attention_fwd: sequences that do not fit). */
 int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k, int max_k,
                           void* k_cache, void* v_cache, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream);
+/* past[b] = the keys of sequence b, 0 where it does not fit `rows` or `longest`: the counts of the tokens that a prompt leaves in a cache */
+int oat_window_cache_counts(int* past, const int* seqs, int B, int rows, int longest, void* stream);
 
 /* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
  * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused; table, if not NULL: the cos and sin of every row's pairs, fp32 [n_pairs, M, 2]), attention with the sequences' query rows as their key rows, out [M, Hq * D]

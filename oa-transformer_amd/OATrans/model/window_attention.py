@@ -152,10 +152,11 @@ class WindowCache:
 
     @torch.no_grad()
     def prompt(self, qkv, seqs, longest, pos=None, scale=None):
-        """Causal attention over the prompts; their keys and values and their counts go into the cache."""
+        """Causal attention over the prompts; their keys and values and their counts go into the cache.  longest: the largest count of
+        the table; a sequence with more is taken as empty, here and in its counts."""
         out = window_attention(qkv, seqs, self.heads, self.kv_heads, self.head_dim, left=self.left, right=0, sinks=self.sinks,
                                longest=longest, scale=scale, rope=self.rope, pos=pos, cache=(self.k, self.v))
-        self.past.copy_(seqs[:, 3])
+        hip.window_cache_counts(self.past, seqs, qkv.shape[0], min(int(longest), qkv.shape[0]))
         return out
 
     @torch.no_grad()

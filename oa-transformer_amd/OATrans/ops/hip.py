@@ -47,6 +47,7 @@ _WINDOW_SIGNATURES = {
     "oat_window_attention_fwd": (_I, [_P, _L, _P, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P] + [_I] * 10 + [_F, _P, _P, ctypes.POINTER(_L), _I, _P]),
     "oat_window_attention_bwd": (_I, [_P, _L, _P, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P, _P, _P] + [_I] * 10 + [_F, _P, _Z, _P]),
     "oat_window_cache_fill": (_I, [_P, _L, _P, _L, _P, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _I, _I, _I, _P]),
+    "oat_window_cache_counts": (_I, [_P, _P, _I, _I, _I, _P]),
 }
 
 
@@ -1207,7 +1208,8 @@ def attn_window_step(qkv, past, k_cache, v_cache, heads, left=-1, sinks=0, rolli
 
 
 def window_cache_fill(k, v, seqs, k_cache, v_cache, max_k, sinks=0):
-    """A prompt's keys and values (rows of seqs) into the caches; more tokens than slots: the sinks and the last ones stay."""
+    """A prompt's keys and values (rows of seqs) into the caches; more tokens than slots: the sinks and the last ones stay.  A sequence
+    with more than max_k tokens, or outside k, leaves its cache as it was."""
     what = "window_cache_fill"
     strides = _cache_args(k_cache, v_cache, what)
     B, cap, kv_heads, D = k_cache.shape
@@ -1219,3 +1221,15 @@ def window_cache_fill(k, v, seqs, k_cache, v_cache, max_k, sinks=0):
     _launch(k.device, lib().oat_window_cache_fill, (
         k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), seqs.data_ptr(), B, k.shape[0], max_k, k_cache.data_ptr(), v_cache.data_ptr(), strides,
         cap, kv_heads, D, _reach(sinks)), "oat_window_cache_fill")
+
+
+def window_cache_counts(past, seqs, rows, longest):
+    """past[b] = the tokens that the prompt of seqs [B, 4] leaves in a cache: its count, 0 for a sequence that does not fit `rows` rows or
+    `longest` tokens (which the attention and the cache leave out)."""
+    what = "window_cache_counts"
+    _need(past.dtype == torch.int32 and past.dim() == 1 and past.is_contiguous(), what + ": past must be a contiguous int32 [B]")
+    _need(seqs.dtype == torch.int32 and seqs.shape == (past.shape[0], 4) and seqs.is_contiguous() and seqs.device == past.device,
+          what + ": seqs must be a contiguous int32 [B, 4] on past's device")
+    _need(0 <= rows < 2 ** 31 and 0 <= longest <= 1 << 29, what + ": rows and the largest count")
+    _launch(past.device, lib().oat_window_cache_counts, (past.data_ptr(), seqs.data_ptr(), past.shape[0], rows, longest), "oat_window_cache_counts")
+    return past

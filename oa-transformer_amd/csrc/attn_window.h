@@ -144,12 +144,12 @@ struct WinArgs {
   const float2* turns;                  // backward: cos and sin of [D / 2, rows_q] pairs (p, p + D / 2) to turn dq and dk back by, or null
 };
 struct Seq { int q0, nq, k0, nk; };
-// a sequence that does not fit the buffers (or the launch) is taken as empty: nothing outside is read or written
+// a sequence that does not fit the buffers (or the launch) is taken as empty, by the attention and by the caches: nothing outside is read or
+// written
+OAT_DEV bool rows_fit(int first, int n, int most, int rows) { return first >= 0 && n >= 0 && n <= most && (long long)first + n <= rows; }
 OAT_DEV Seq load_seq(const WinArgs& a, int b) {
   const int4 s = a.seqs[b];
-  const bool ok = s.x >= 0 && s.y >= 0 && s.z >= 0 && s.w >= 0 && s.y <= a.max_q && s.w <= a.max_k && (long long)s.x + s.y <= a.rows_q &&
-                  (long long)s.z + s.w <= a.rows_k;
-  return ok ? Seq{s.x, s.y, s.z, s.w} : Seq{0, 0, 0, 0};
+  return rows_fit(s.x, s.y, a.max_q, a.rows_q) && rows_fit(s.z, s.w, a.max_k, a.rows_k) ? Seq{s.x, s.y, s.z, s.w} : Seq{0, 0, 0, 0};
 }
 // blockIdx -> (tile, head, sequence).  Workgroups go to the 8 XCDs in turn; the (sequence, head, tile) list is dealt to the XCDs in runs of
 // a.run tiles, which share keys in one L2 (deal_run below).

@@ -296,12 +296,13 @@ struct FillArgs {
   char *kc, *vc;
   long long kb, ks, kh, vb, vs, vh;
   const int4* seqs;
-  int B, Hkv, cap, sinks, rows_k, chunks;            // chunks: 16-byte pieces of a head
+  int B, Hkv, cap, sinks, rows_k, max_k, chunks;     // chunks: 16-byte pieces of a head
+  int rows_q, max_q;                                 // the attention's, where the prompt's queries have to fit too; max_q < 0: they need not
 };
 __global__ __launch_bounds__(256) void cache_fill_kernel(FillArgs a) {
   const int b = blockIdx.y, per = a.Hkv * a.chunks;
   const int4 s = a.seqs[b];
-  if (s.z < 0 || s.w < 0 || (long long)s.z + s.w > a.rows_k) return;
+  if (!rows_fit(s.z, s.w, a.max_k, a.rows_k) || (a.max_q >= 0 && !rows_fit(s.x, s.y, a.max_q, a.rows_q))) return;
   const int S = min(a.sinks, a.cap), W = a.cap - S;
   const long long total = (long long)min(a.cap, s.w) * per;
   for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
@@ -392,9 +393,8 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
   return check_launch(me);
 }
 
-extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k,
-                                     int max_k, void* kc, void* vc, const long long* strides, int cap, int Hkv, int D, int sinks,
-                                     void* stream) {
+static int cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k, int max_k, int rows_q,
+                      int max_q, void* kc, void* vc, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream) {
   const char* me = "window_cache_fill";
   if (B == 0) return 0;
   if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
@@ -406,9 +406,33 @@ extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v
   a.k = (const char*)k; a.v = (const char*)v; a.ldk = ldk * 2; a.ldv = ldv * 2; a.kc = (char*)kc; a.vc = (char*)vc;
   a.kb = strides[0] * 2; a.ks = strides[1] * 2; a.kh = strides[2] * 2; a.vb = strides[3] * 2; a.vs = strides[4] * 2; a.vh = strides[5] * 2;
   a.seqs = (const int4*)seqs;
-  a.B = B; a.Hkv = Hkv; a.cap = cap; a.sinks = sinks; a.rows_k = rows_k; a.chunks = D / 8;
+  a.B = B; a.Hkv = Hkv; a.cap = cap; a.sinks = sinks; a.rows_k = rows_k; a.max_k = max_k; a.chunks = D / 8;
+  a.rows_q = rows_q; a.max_q = max_q;
   const long long n = (long long)min(cap, max_k) * Hkv * a.chunks;
   OAT_LAUNCH(cache_fill_kernel, dim3((unsigned)min((n + 255) / 256, 4096ll), B), dim3(256), 0, (hipStream_t)stream, a);
+  return check_launch(me);
+}
+
+extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long ldv, const int* seqs, int B, int rows_k,
+                                     int max_k, void* kc, void* vc, const long long* strides, int cap, int Hkv, int D, int sinks,
+                                     void* stream) {
+  return cache_fill(k, ldk, v, ldv, seqs, B, rows_k, max_k, 0, -1, kc, vc, strides, cap, Hkv, D, sinks, stream);
+}
+
+// ---- the counts of tokens that belong to a cache: those of a prompt, by the rule that the attention and the fill go by
+static __global__ __launch_bounds__(256) void cache_counts_kernel(int* past, const int4* seqs, int B, int rows, int longest) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int4 s = seqs[b];
+  past[b] = rows_fit(s.x, s.y, longest, rows) && rows_fit(s.z, s.w, longest, rows) ? s.w : 0;
+}
+
+extern "C" int oat_window_cache_counts(int* past, const int* seqs, int B, int rows, int longest, void* stream) {
+  const char* me = "window_cache_counts";
+  if (B < 0 || rows < 0 || longest < 0) return fail(me, "a negative number of sequences, rows or tokens");
+  if (B == 0) return 0;
+  if (!past || !seqs || (uintptr_t)seqs % 16) return fail(me, "the counts, or the table of sequences (on 16 bytes), are missing");
+  OAT_LAUNCH(cache_counts_kernel, dim3((B + 255) / 256), dim3(256), 0, (hipStream_t)stream, past, (const int4*)seqs, B, rows, longest);
   return check_launch(me);
 }
 
@@ -438,7 +462,7 @@ extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* tur
   const char* k = M ? q + a * 2 : q;
   if (int rc = oat_attn_window_fwd(q, ldq, k, ldq, v, ld, out, a, lse, seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks,
                                    scale, stream)) return rc;
-  return kc ? oat_window_cache_fill(k, ldq, v, ld, seqs, B, M, longest, kc, vc, strides, cap, Hkv, D, sinks, stream) : 0;
+  return kc ? cache_fill(k, ldq, v, ld, seqs, B, M, longest, M, longest, kc, vc, strides, cap, Hkv, D, sinks, stream) : 0;
 }
 
 extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period,

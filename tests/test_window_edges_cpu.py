@@ -1,0 +1,32 @@
+"""Refusals of the windowed attention's entry points, each by its own message, and the caches' checks: no GPU is needed."""
+import ctypes
+
+import pytest
+import torch
+
+LL = ctypes.c_longlong
+
+
+def _hip():
+    from OATrans.ops import hip
+    hip.lib()
+    return hip
+
+
+def _refused(hip, rc, text):
+    assert rc < 0 and text in hip.lib().oat_last_error(), hip.lib().oat_last_error()
+
+
+def test_counts_refusals():
+    hip = _hip()
+    counts = lambda past=4096, seqs=4096, B=1, rows=10, longest=10: hip.lib().oat_window_cache_counts(past, seqs, B, rows, longest, None)
+    for change in (dict(B=-1), dict(rows=-1), dict(longest=-1)):
+        _refused(hip, counts(**change), b"negative")
+    for change in (dict(past=None), dict(seqs=None), dict(seqs=4100)):
+        _refused(hip, counts(**change), b"missing")
+    assert counts(B=0) == 0
+    past, seqs = torch.zeros(2, dtype=torch.int32), hip.seq_table([1, 2], device="cpu")
+    for p, s, rows, longest, text in ((past.long(), seqs, 3, 2, "past must"), (past[:1], seqs, 3, 2, "seqs must"), (past, seqs.long(), 3, 2, "seqs must"),
+                                      (past, seqs, -1, 2, "rows"), (past, seqs, 3, 2 ** 30, "largest"), (past, seqs, 3, 2, "no CPU path")):
+        with pytest.raises(hip.OatError, match=text):
+            hip.window_cache_counts(p, s, rows, longest)

@@ -1,0 +1,45 @@
+"""Calls of the windowed attention, its caches and rotary positions at the edges of what their documentation allows, on a real MI355X
+against their definitions in 64 bits (oracle/window_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+from oracle import window_oracle as wo
+from tests.test_window_gpu import BF, DEV, HF, _hip, half_step, rnd, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- a table that understates its longest count
+@pytest.mark.parametrize("window,slots,sinks", [(None, 20, 0), (9, None, 2)])
+def test_cache_and_attention_leave_out_the_same_sequences(window, slots, sinks):
+    """A sequence with more tokens than `longest` is taken as empty: by the attention, the cache and the cache's counts alike."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    lens, D = [7, 13, 5], 64
+    qkv, table = rnd(sum(lens), 3 * D, seed=2), hip.seq_table(lens)
+    cache = wa.WindowCache(3, 1, 1, D, window=window, sinks=sinks, slots=slots)
+    cache.k.fill_(7.0), cache.v.fill_(7.0)
+    out = cache.prompt(qkv, table, 10)
+    ok = wa.WindowCache(3, 1, 1, D, window=window, sinks=sinks, slots=slots)
+    ok.k.fill_(7.0), ok.v.fill_(7.0)
+    ref = ok.prompt(qkv, hip.seq_table([7, 0, 5], q_rows=(0, 7, 20)), 10)
+    assert (out[7:20] == 0).all() and torch.equal(out, ref)
+    assert torch.equal(cache.k, ok.k) and torch.equal(cache.v, ok.v) and (cache.k[1] == 7.0).all()
+    assert cache.past.tolist() == ok.past.tolist() == [7, 0, 5]
+    # the next token of the sequence that was left out is its first
+    x = rnd(3, 3 * D, seed=3)
+    assert torch.equal(cache.step(x)[1], x[1, 2 * D:]) and cache.past.tolist() == [8, 1, 6]
+
+
+def test_counts_of_tables_that_do_not_fit_are_zero():
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    qkv = rnd(30, 192)
+    for bad in ((-1, 5, 0, 5), (28, 5, 28, 5), (0, 5, 26, 5), (0, 11, 0, 11), (0, -1, 0, 5), (2 ** 31 - 4, 5, 0, 5), (0, 5, 2 ** 31 - 4, 5)):
+        cache = wa.WindowCache(2, 1, 1, 64, slots=12)
+        table = torch.tensor([bad, (20, 6, 20, 6)], dtype=torch.int32, device=DEV)
+        out = cache.prompt(qkv, table, 10)
+        assert cache.past.tolist() == [0, 6] and (cache.k[0] == 0).all() and (cache.v[0] == 0).all() and (out[:20] == 0).all()
+        assert torch.equal(cache.v[1, :6, 0], qkv[20:26, 128:]) and (cache.v[1, 6:] == 0).all()
