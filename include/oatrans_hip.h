@@ -332,6 +332,8 @@ int oat_window_cache_fill(const void* k, long long ldk, const void* v, long long
                           void* k_cache, void* v_cache, const long long* strides, int cap, int Hkv, int D, int sinks, void* stream);
 /* past[b] = the keys of sequence b, 0 where it does not fit `rows` or `longest`: the counts of the tokens that a prompt leaves in a cache */
 int oat_window_cache_counts(int* past, const int* seqs, int B, int rows, int longest, void* stream);
+/* after a step: one token more for every sequence that took part (0 <= past[b] < cap; cap < 0, a rolling cache: past[b] >= 0) */
+int oat_window_cache_advance(int* past, int B, int cap, void* stream);
 
 /* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
  * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused; table, if not NULL: the cos and sin of every row's pairs, fp32 [n_pairs, M, 2]), attention with the sequences' query rows as their key rows, out [M, Hq * D]

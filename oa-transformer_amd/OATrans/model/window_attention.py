@@ -137,7 +137,8 @@ class WindowCache:
     """Keys and values of B sequences that are written token by token, with the operator's workspace and the counts of tokens.
 
     window: tokens that stay visible besides the `sinks` first ones; the cache then holds sinks + window slots and rolls.  None: it
-    holds `slots` tokens and everything is visible."""
+    holds `slots` tokens and everything is visible; a sequence without a slot left takes no part any more: step gives it a row of
+    zeros, and its cache and its count (past == slots) stay.  past may be set by the caller: a negative count takes no part either."""
 
     def __init__(self, B, heads, kv_heads, head_dim, window=None, sinks=0, slots=None, rope=None, dtype=torch.bfloat16, device="cuda"):
         if (window is None) == (slots is None) or (window is not None and window < 1) or (slots is not None and slots < 1):
@@ -169,5 +170,5 @@ class WindowCache:
             pos = self.past[:, None]
         out = hip.attn_window_step(qkv, self.past, self.k, self.v, self.heads, left=self.left, sinks=self.sinks, rolling=self.rolling,
                                    scale=scale, rope=self.rope, pos=pos, pieces=self.pieces)
-        self.past += self.past >= 0
+        hip.window_cache_advance(self.past, None if self.rolling else self.slots)
         return out

@@ -48,6 +48,7 @@ _WINDOW_SIGNATURES = {
     "oat_window_attention_bwd": (_I, [_P, _L, _P, _P, ctypes.POINTER(_OatRope), _P, _I, _P, _P, _P, _P, _P] + [_I] * 10 + [_F, _P, _Z, _P]),
     "oat_window_cache_fill": (_I, [_P, _L, _P, _L, _P, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _I, _I, _I, _P]),
     "oat_window_cache_counts": (_I, [_P, _P, _I, _I, _I, _P]),
+    "oat_window_cache_advance": (_I, [_P, _I, _I, _P]),
 }
 
 
@@ -1232,4 +1233,13 @@ def window_cache_counts(past, seqs, rows, longest):
           what + ": seqs must be a contiguous int32 [B, 4] on past's device")
     _need(0 <= rows < 2 ** 31 and 0 <= longest <= 1 << 29, what + ": rows and the largest count")
     _launch(past.device, lib().oat_window_cache_counts, (past.data_ptr(), seqs.data_ptr(), past.shape[0], rows, longest), "oat_window_cache_counts")
+    return past
+
+
+def window_cache_advance(past, slots=None):
+    """After attn_window_step: one token more for every sequence that took part (past >= 0 and, in a plain cache of `slots`, a slot left)."""
+    what = "window_cache_advance"
+    _need(past.dtype == torch.int32 and past.dim() == 1 and past.is_contiguous(), what + ": past must be a contiguous int32 [B]")
+    _need(slots is None or 1 <= slots < 2 ** 31, what + ": at least one of the slots")
+    _launch(past.device, lib().oat_window_cache_advance, (past.data_ptr(), past.shape[0], -1 if slots is None else slots), "oat_window_cache_advance")
     return past

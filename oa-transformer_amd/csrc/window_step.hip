@@ -419,7 +419,8 @@ extern "C" int oat_window_cache_fill(const void* k, long long ldk, const void* v
   return cache_fill(k, ldk, v, ldv, seqs, B, rows_k, max_k, 0, -1, kc, vc, strides, cap, Hkv, D, sinks, stream);
 }
 
-// ---- the counts of tokens that belong to a cache: those of a prompt, by the rule that the attention and the fill go by
+// ---- the counts of tokens that belong to a cache: those of a prompt, by the rule that the attention and the fill go by, and a step's, by
+// the rule that the step goes by (in a launch of its own: a step's workgroups read the counts as long as any of them runs)
 static __global__ __launch_bounds__(256) void cache_counts_kernel(int* past, const int4* seqs, int B, int rows, int longest) {
   const int b = blockIdx.x * 256 + threadIdx.x;
   if (b >= B) return;
@@ -433,6 +434,22 @@ extern "C" int oat_window_cache_counts(int* past, const int* seqs, int B, int ro
   if (B == 0) return 0;
   if (!past || !seqs || (uintptr_t)seqs % 16) return fail(me, "the counts, or the table of sequences (on 16 bytes), are missing");
   OAT_LAUNCH(cache_counts_kernel, dim3((B + 255) / 256), dim3(256), 0, (hipStream_t)stream, past, (const int4*)seqs, B, rows, longest);
+  return check_launch(me);
+}
+
+static __global__ __launch_bounds__(256) void cache_advance_kernel(int* past, int B, int cap) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int p = past[b];
+  if (p >= 0 && p < cap) past[b] = p + 1;
+}
+
+extern "C" int oat_window_cache_advance(int* past, int B, int cap, void* stream) {
+  const char* me = "window_cache_advance";
+  if (B < 0) return fail(me, "a negative number of sequences");
+  if (B == 0) return 0;
+  if (!past) return fail(me, "the counts are missing");
+  OAT_LAUNCH(cache_advance_kernel, dim3((B + 255) / 256), dim3(256), 0, (hipStream_t)stream, past, B, cap < 0 ? 0x7fffffff : cap);
   return check_launch(me);
 }
 

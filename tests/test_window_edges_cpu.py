@@ -30,3 +30,14 @@ def test_counts_refusals():
                                       (past, seqs, -1, 2, "rows"), (past, seqs, 3, 2 ** 30, "largest"), (past, seqs, 3, 2, "no CPU path")):
         with pytest.raises(hip.OatError, match=text):
             hip.window_cache_counts(p, s, rows, longest)
+
+
+def test_advance_refusals():
+    hip = _hip()
+    _refused(hip, hip.lib().oat_window_cache_advance(4096, -1, 8, None), b"negative")
+    _refused(hip, hip.lib().oat_window_cache_advance(None, 1, 8, None), b"missing")
+    assert hip.lib().oat_window_cache_advance(None, 0, 8, None) == 0
+    past = torch.zeros(2, dtype=torch.int32)
+    for p, slots, text in ((past.long(), 8, "past must"), (past[:, None], 8, "past must"), (past, 0, "slots"), (past, 2 ** 31, "slots"), (past, 8, "no CPU path")):
+        with pytest.raises(hip.OatError, match=text):
+            hip.window_cache_advance(p, slots)

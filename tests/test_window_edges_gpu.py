@@ -43,3 +43,25 @@ def test_counts_of_tables_that_do_not_fit_are_zero():
         out = cache.prompt(qkv, table, 10)
         assert cache.past.tolist() == [0, 6] and (cache.k[0] == 0).all() and (cache.v[0] == 0).all() and (out[:20] == 0).all()
         assert torch.equal(cache.v[1, :6, 0], qkv[20:26, 128:]) and (cache.v[1, 6:] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------- counts
+def test_a_full_cache_stops_counting():
+    """A plain cache without a slot left: its row is zero, the cache and the count stay; the others go on, and so does one that
+    takes no part."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    cache = wa.WindowCache(4, 2, 1, 64, slots=6)
+    cache.past.copy_(torch.tensor([4, 0, -1, 6], dtype=torch.int32))
+    for t in range(4):
+        held = cache.k.clone(), cache.v.clone()
+        x = rnd(4, 4 * 64, seed=t)
+        out = cache.step(x)
+        assert cache.past.tolist() == [min(5 + t, 6), 1 + t, -1, 6]
+        assert (out[2:] == 0).all() and (out[1] != 0).any() and (out[0] == 0).all() == (t >= 2)
+        for c, h in zip((cache.k, cache.v), held):
+            assert torch.equal(c[2:], h[2:]) and torch.equal(c[0], h[0]) == (t >= 2)
+    rolling = wa.WindowCache(3, 1, 1, 64, window=4, sinks=1)
+    rolling.past.copy_(torch.tensor([2 ** 31 - 1, 9, -5], dtype=torch.int32))
+    rolling.step(rnd(3, 192))
+    assert rolling.past.tolist() == [2 ** 31 - 1, 10, -5]              # (the largest count is not passed)
