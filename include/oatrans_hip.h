@@ -337,7 +337,8 @@ int oat_window_cache_advance(int* past, int B, int cap, void* stream);
 
 /* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
  * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused; table, if not NULL: the cos and sin of every row's pairs, fp32 [n_pairs, M, 2]), attention with the sequences' query rows as their key rows, out [M, Hq * D]
- * dense, and - with k_cache - the prompt's cache.  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back (with the forward's table, of
+ * dense, and - with k_cache - the prompt's cache.  A sequence that is left out because it has more than `longest` tokens gets zeros, both
+ * ways (but for longest = 0: nothing is written).  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back (with the forward's table, of
  * pairs that are a head's two halves, before its rounding; else in a pass of its own); workspace as for
  * oat_attn_window_bwd with max_q = max_k = longest. */
 int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out, float* lse,

@@ -33,6 +33,11 @@ def rope_axes(x, pos, rope, heads, head_dim):
     return _RopeFn.apply(x, pos, rope, heads, head_dim)
 
 
+def _new(packed, longest, seqs):
+    """how a result starts: the library writes the rows of every sequence whose rows lie in the buffer, where there is any work"""
+    return torch.empty if packed and longest > 0 and seqs.shape[0] else torch.zeros
+
+
 def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, packed, lse, cache):
     """-> (out, turned q | k or None, the turns or None): rotary positions into a new buffer (the values stay where they are), attention
     over it, and the prompt's rows into the cache, in one call.  The turns - every row's cos and sin - are kept for a backward pass
@@ -52,7 +57,7 @@ def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, p
         turned, struct, places, period = qk.data_ptr(), rope.struct, pos.data_ptr(), pos.shape[0]
         if lse is not None and 2 * rope.pairs == D and not rope.interleaved:
             turns = torch.empty(rope.pairs, M, 2, dtype=torch.float32, device=dev)
-    out = (torch.empty if packed else torch.zeros)(M, heads * D, dtype=dt, device=dev)
+    out = _new(packed, longest, seqs)(M, heads * D, dtype=dt, device=dev)
     kc = vc = strides = None
     cap = 0
     if cache is not None:
@@ -89,7 +94,7 @@ class _WindowFn(torch.autograd.Function):
         if dout.data_ptr() % 16:
             dout = dout.clone()
         M, B = qkv.shape[0], seqs.shape[0]
-        dqkv = (torch.empty if packed else torch.zeros)(qkv.shape, dtype=qkv.dtype, device=dev)
+        dqkv = _new(packed, longest, seqs)(qkv.shape, dtype=qkv.dtype, device=dev)
         need = lib.oat_attn_window_bwd_workspace_bytes(M, B, longest, longest, heads, kv_heads, D, window[0], window[2])
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         hip._launch(dev, lib.oat_window_attention_bwd, (
@@ -105,7 +110,8 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
                      packed=False, cache=None):
     """qkv [M, (heads + 2 * kv_heads) * head_dim] (bf16 / fp16; q | k | v) -> [M, heads * head_dim].
 
-    seqs: int32 [B, 4] on the device (hip.seq_table); longest: the largest count in it (default: M).  Token i of a sequence sees
+    seqs: int32 [B, 4] on the device (hip.seq_table); longest: the largest count in it (default: M; a sequence with more is taken as
+    empty: zeros).  Token i of a sequence sees
     token j if j <= i + right and (j >= i - left or j < sinks); left / right < 0: no such edge, right = 0: causal.
     rope, pos: rotary positions of q and k, pos int32 [P, axes] with M a multiple of P.
     packed: the caller states that every row belongs to a sequence; otherwise rows of none (padding) get zeros, and zero gradients.

@@ -141,15 +141,25 @@ struct WinArgs {
   int run;                              // tiles that go to one XCD together
   int groups, pieces, far_blocks;       // how the sinks' far queries are split; their workgroups in the launch
   float scale;
+  int clear;                            // rows of a sequence that is left out for its length get zeros (the layer's do)
   const float2* turns;                  // backward: cos and sin of [D / 2, rows_q] pairs (p, p + D / 2) to turn dq and dk back by, or null
 };
 struct Seq { int q0, nq, k0, nk; };
 // a sequence that does not fit the buffers (or the launch) is taken as empty, by the attention and by the caches: nothing outside is read or
 // written
 OAT_DEV bool rows_fit(int first, int n, int most, int rows) { return first >= 0 && n >= 0 && n <= most && (long long)first + n <= rows; }
+OAT_DEV bool left_out(const WinArgs& a, const int4& s) { return !(rows_fit(s.x, s.y, a.max_q, a.rows_q) && rows_fit(s.z, s.w, a.max_k, a.rows_k)); }
 OAT_DEV Seq load_seq(const WinArgs& a, int b) {
   const int4 s = a.seqs[b];
-  return rows_fit(s.x, s.y, a.max_q, a.rows_q) && rows_fit(s.z, s.w, a.max_k, a.rows_k) ? Seq{s.x, s.y, s.z, s.w} : Seq{0, 0, 0, 0};
+  return left_out(a, s) ? Seq{0, 0, 0, 0} : Seq{s.x, s.y, s.z, s.w};
+}
+// Zeros for head h's rows of a sequence that load_seq left out though its rows lie in the buffer (there are more than stated, or its other
+// side does not fit): the caller's buffer may be a new one, and no other workgroup writes them.  `part` of `parts` workgroups.
+template <int D> OAT_DEV void clear_rows(char* base, long long ld, int first, int n, int rows, int h, int part, int parts) {
+  if (!rows_fit(first, n, n, rows)) return;
+  constexpr int CPR = D / 8;
+  for (long long t = part * 256 + (int)threadIdx.x; t < (long long)n * CPR; t += parts * 256)
+    *reinterpret_cast<f32x4*>(base + (first + t / CPR) * ld + h * (D * 2) + t % CPR * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 // blockIdx -> (tile, head, sequence).  Workgroups go to the 8 XCDs in turn; the (sequence, head, tile) list is dealt to the XCDs in runs of
 // a.run tiles, which share keys in one L2 (deal_run below).
@@ -225,10 +235,14 @@ OAT_DEV KeyTiles key_tiles(const WinArgs& a, int nk, int p0, int p1) {
   return {sink, first, sink + max(0, end - first)};
 }
 
-// oat_attn_window_bwd; `turns` (may be null): dq and dk are turned back by these before they are rounded (WinArgs::turns; rows_q = rows_k)
+// oat_attn_window_fwd and _bwd; clear: WinArgs::clear; `turns` (may be null): dq and dk are turned back by these before they are rounded
+// (WinArgs::turns; rows_q = rows_k)
+int attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
+                    float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
+                    int left, int right, int sinks, float scale, int clear, void* stream);
 int attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out, long long ldo,
                     const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk, long long lddk, void* dv,
                     long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
-                    int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, const float2* turns, void* stream);
+                    int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, const float2* turns, int clear, void* stream);
 
 }  // namespace oat

@@ -22,7 +22,10 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   if (!place(a, tiles, a.Hq, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int i0 = (tiles - 1 - pl.tile) * 128;                          // causal rows are longest at the end: those first
-  if (i0 >= s.nq) return;
+  if (i0 >= s.nq) {
+    if (const int4 t = a.seqs[pl.b]; a.clear && left_out(a, t)) clear_rows<D>(a.out, a.ldo, t.x, t.y, a.rows_q, pl.h, pl.tile, tiles);
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int off = s.nk - s.nq, hk = pl.h / (a.Hq / a.Hkv);
   const KeyTiles kt = key_tiles(a, s.nk, i0 + off, min(i0 + 127, s.nq - 1) + off);
@@ -242,7 +245,10 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   if (!place(a, tiles, a.Hq, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int i0 = (tiles - 1 - pl.tile) * 128;
-  if (i0 >= s.nq) return;
+  if (i0 >= s.nq) {
+    if (const int4 t = a.seqs[pl.b]; a.clear && left_out(a, t)) clear_rows<D>(a.dq, a.lddq, t.x, t.y, a.rows_q, pl.h, pl.tile, tiles);
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int off = s.nk - s.nq, hk = pl.h / (a.Hq / a.Hkv);
   const KeyTiles kt = key_tiles(a, s.nk, i0 + off, min(i0 + 127, s.nq - 1) + off);
@@ -445,6 +451,13 @@ template <class T, int D> OAT_DEV void far_keys(const WinArgs& a, char* lds, int
     for (int r = 0; r < 16; ++r) sl[(dt * 32 + 8 * (r >> 2) + 4 * half + (r & 3)) * 32] = sum[dt][r];
 }
 
+template <int D> OAT_DEV void clear_keys(const WinArgs& a, const Place& pl, int tiles) {
+  const int4 t = a.seqs[pl.b];
+  if (!left_out(a, t)) return;
+  clear_rows<D>(a.dk, a.lddk, t.z, t.w, a.rows_k, pl.h, pl.tile, tiles);
+  clear_rows<D>(a.dv, a.lddv, t.z, t.w, a.rows_k, pl.h, pl.tile, tiles);
+}
+
 // 128 keys, 32 a wave: S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and their gradients
 // pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: instruction issue (four products for one exponential): the
 // clips of above 180 us = 797 TFLOP/s.
@@ -452,10 +465,14 @@ template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) 
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
   Place pl;
-  if (!place(a, (a.max_k + 127) / 128, a.Hkv, pl)) return;
+  const int tiles = (a.max_k + 127) / 128;
+  if (!place(a, tiles, a.Hkv, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int j0 = pl.tile * 128;
-  if (j0 >= s.nk) return;
+  if (j0 >= s.nk) {
+    if (a.clear) clear_keys<D>(a, pl, tiles);
+    return;
+  }
   const int off = s.nk - s.nq;
   const bool split = a.groups > 0;                                     // the sinks' far queries are other workgroups' (far_keys)
   // the queries that see key j: i = lo(j) .. hi(j)
@@ -566,10 +583,14 @@ template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, ch
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
   Place pl;
-  if (!place(a, (a.max_k + 63) / 64, a.Hkv, pl)) return;
+  const int tiles = (a.max_k + 63) / 64;
+  if (!place(a, tiles, a.Hkv, pl)) return;
   const Seq s = load_seq(a, pl.b);
   const int j0 = pl.tile * 64;
-  if (j0 >= s.nk) return;
+  if (j0 >= s.nk) {
+    if (a.clear) clear_keys<D>(a, pl, tiles);
+    return;
+  }
   const int off = s.nk - s.nq;
   const bool split = a.groups > 0;                                     // the sinks' far queries are other workgroups' (far_keys)
   auto lo = [&](int j) WIN_INLINE { return j - a.right - off; };       // the queries that see key j
@@ -806,9 +827,9 @@ using namespace oat;
     else OAT_LAUNCH((kernel(_Float16, 128)), g_, dim3(256), 0, s, a);                                                  \
   } while (0)
 
-extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
-                                   long long ldo, float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k,
-                                   int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* stream) {
+int oat::attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
+                         float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
+                         int left, int right, int sinks, float scale, int clear, void* stream) {
   if (int rc = window_wrong("attn_window_fwd", seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, sinks, scale)) return rc;
   if (B == 0 || max_q == 0 || rows_q == 0) return 0;
   if (rows_wrong(q, ldq, Hq, D) || rows_wrong(out, ldo, Hq, D) || (rows_k && (rows_wrong(k, ldk, Hkv, D) || rows_wrong(v, ldv, Hkv, D)))) {
@@ -820,12 +841,19 @@ extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, 
   a.ldq = ldq * 2; a.ldk = ldk * 2; a.ldv = ldv * 2; a.ldo = ldo * 2;
   a.seqs = (const int4*)seqs;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
-  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
+  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale; a.clear = clear;
   hipStream_t s = (hipStream_t)stream;
   const int tiles = (max_q + 127) / 128;
   a.run = deal_run(B, Hq, Hq / Hkv, tiles, rows_q, max_q);
   WIN_LAUNCH(WIN_FWD, deal_grid((long long)B * Hq * tiles, a.run));
   return check_launch("attn_window_fwd");
+}
+
+extern "C" int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
+                                   long long ldo, float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k,
+                                   int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* stream) {
+  return attn_window_fwd(q, ldq, k, ldk, v, ldv, out, ldo, lse, seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, left, right, sinks,
+                         scale, 0, stream);
 }
 
 extern "C" size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max_q, int max_k, int Hq, int Hkv, int D, int left, int sinks) {
@@ -837,7 +865,7 @@ int oat::attn_window_bwd(const void* q, long long ldq, const void* k, long long 
                          long long ldo, const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk,
                          long long lddk, void* dv, long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k,
                          int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
-                         size_t workspace_bytes, const float2* turns, void* stream) {
+                         size_t workspace_bytes, const float2* turns, int clear, void* stream) {
   if (int rc = window_wrong("attn_window_bwd", seqs, B, max_q, max_k, rows_q, rows_k, Hq, Hkv, D, dtype, sinks, scale)) return rc;
   if (B == 0) return 0;
   if (rows_q && (rows_wrong(q, ldq, Hq, D) || rows_wrong(out, ldo, Hq, D) || rows_wrong(dout, lddo, Hq, D) || rows_wrong(dq, lddq, Hq, D) || !lse)) {
@@ -856,7 +884,7 @@ int oat::attn_window_bwd(const void* q, long long ldq, const void* k, long long 
   a.lse2 = (float*)workspace; a.delta = a.lse2 + (size_t)rows_q * Hq;
   a.seqs = (const int4*)seqs;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.left = far(left); a.right = far(right); a.sinks = sinks;
-  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale;
+  a.max_q = max_q; a.max_k = max_k; a.rows_q = rows_q; a.rows_k = rows_k; a.scale = scale; a.clear = clear;
   a.turns = turns;
   hipStream_t s = (hipStream_t)stream;
   if (max_q && rows_q) {
@@ -884,5 +912,5 @@ extern "C" int oat_attn_window_bwd(const void* q, long long ldq, const void* k, 
                                    int rows_k, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale,
                                    void* workspace, size_t workspace_bytes, void* stream) {
   return attn_window_bwd(q, ldq, k, ldk, v, ldv, out, ldo, lse, dout, lddo, dq, lddq, dk, lddk, dv, lddv, seqs, B, max_q, max_k, rows_q, rows_k,
-                         Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes, nullptr, stream);
+                         Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes, nullptr, 0, stream);
 }

@@ -477,8 +477,8 @@ extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* tur
     ldq = n;
   }
   const char* k = M ? q + a * 2 : q;
-  if (int rc = oat_attn_window_fwd(q, ldq, k, ldq, v, ld, out, a, lse, seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks,
-                                   scale, stream)) return rc;
+  if (int rc = attn_window_fwd(q, ldq, k, ldq, v, ld, out, a, lse, seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks,
+                               scale, 1, stream)) return rc;
   return kc ? cache_fill(k, ldq, v, ld, seqs, B, M, longest, M, longest, kc, vc, strides, cap, Hkv, D, sinks, stream) : 0;
 }
 
@@ -498,6 +498,6 @@ extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const voi
   if (turns && (uintptr_t)table % 8) return fail("window_attention_bwd", "the table of the turns is not aligned to 8 bytes");
   if (int rc = attn_window_bwd(q, ldq, q + a * 2, ldq, (const char*)qkv + n * 2, ld, out, a, lse, dout, a, g, w, g + a * 2, w, g + n * 2, w,
                                    seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes,
-                               turns, stream)) return rc;
+                               turns, 1, stream)) return rc;
   return rope && !turns ? oat_rope_axes(g, w, g, w, dtype, pos, period, M, Hq + Hkv, D, rope, 1, stream) : 0;
 }

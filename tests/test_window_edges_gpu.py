@@ -65,3 +65,32 @@ def test_a_full_cache_stops_counting():
     rolling.past.copy_(torch.tensor([2 ** 31 - 1, 9, -5], dtype=torch.int32))
     rolling.step(rnd(3, 192))
     assert rolling.past.tolist() == [2 ** 31 - 1, 10, -5]              # (the largest count is not passed)
+
+
+# ---------------------------------------------------------------------------------------------- rows without a result
+@pytest.mark.parametrize("D,Hq,Hkv,longest,lens", [(64, 2, 1, 10, [7, 13, 5]), (128, 4, 2, 200, [200, 901, 1]), (64, 3, 3, 0, [4, 9]), (128, 1, 1, 3, [])])
+@pytest.mark.parametrize("packed", [True, False])
+def test_rows_of_a_sequence_that_is_left_out_are_zeros(D, Hq, Hkv, longest, lens, packed):
+    """With packed=True the results are new memory that the kernels fill: also for a sequence that has more tokens than `longest`."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    M, W = max(30, sum(lens)) if not lens else sum(lens), (Hq + 2 * Hkv) * D
+    qkv, dout, table = rnd(M, W, seed=5).requires_grad_(), rnd(M, Hq * D, seed=6), hip.seq_table(lens)
+
+    def dirty():
+        for width in (Hq * D, W):                                        # what the allocator hands out next
+            for t in [torch.full((M, width), 7.0, dtype=BF, device=DEV) for _ in range(3)]:
+                del t
+    dirty()
+    out = wa.window_attention(qkv, table, Hq, Hkv, D, 50, 0, 1, longest=longest, packed=packed)
+    dirty()
+    (g,) = torch.autograd.grad(out, qkv, dout)
+    kept = [n if n <= longest else 0 for n in lens]
+    starts = [sum(lens[:b]) for b in range(len(lens))]
+    ref = wa.window_attention(qkv, hip.seq_table(kept, q_rows=starts), Hq, Hkv, D, 50, 0, 1, longest=longest)
+    (gr,) = torch.autograd.grad(ref, qkv, dout)
+    assert torch.equal(out, ref) and torch.equal(g, gr)
+    own = torch.zeros(M, dtype=torch.bool, device=DEV)
+    for at, n in zip(starts, kept):
+        own[at:at + n] = True
+    assert (out[~own] == 0).all() and (g[~own] == 0).all() and (out[own] != 0).any(1).all()
