@@ -212,7 +212,8 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   for (; n < kt.count; ++n) turn(n, n & 1);
   if (i >= s.nq) return;
   l = both_halves(l, false);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  // 0: the row sees nothing (of a row that sees a key the reference's own term is 1); not a number: that is what out and lse say
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   char* po = a.out + (long long)(s.q0 + i) * a.ldo + pl.h * (D * 2);
   typedef __attribute__((ext_vector_type(4))) T T4;
 #pragma unroll
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
       for (int e = 0; e < 4; ++e) y[e] = (T)(o[dt][4 * g + e] * inv);
       *reinterpret_cast<T4*>(po + (dt * 32 + 8 * g + 4 * half) * 2) = y;
     }
-  if (a.lse && half == 0) a.lse[(size_t)(s.q0 + i) * a.Hq + pl.h] = l > 0.f ? (__log2f(l) - neg) * LN2 : -INFINITY;
+  if (a.lse && half == 0) a.lse[(size_t)(s.q0 + i) * a.Hq + pl.h] = l == 0.f ? -INFINITY : (__log2f(l) - neg) * LN2;
 }
 
 // ---------------------------------------------------------------------------------------------- backward
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
     delta = both_halves(delta, false);
   }
   float lse2 = a.lse[(size_t)row * a.Hq + pl.h] * LOG2E;
-  if (!(lse2 > -INFINITY)) lse2 = 0.f;                                 // a row that sees nothing: every pair of it is masked below
+  if (lse2 == -INFINITY) lse2 = 0.f;                                   // a row that sees nothing: every pair of it is masked below
   if (i < s.nq && half == 0) {
     a.lse2[(size_t)pl.h * a.rows_q + row] = lse2;
     a.delta[(size_t)pl.h * a.rows_q + row] = delta;

@@ -94,3 +94,28 @@ def test_rows_of_a_sequence_that_is_left_out_are_zeros(D, Hq, Hkv, longest, lens
     for at, n in zip(starts, kept):
         own[at:at + n] = True
     assert (out[~own] == 0).all() and (g[~own] == 0).all() and (out[own] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_what_is_not_a_number_shows(D, dtype):
+    """A query or key that is not a number: the rows it belongs to say so, in out, in lse and in their gradient; lse = -inf is said by rows
+    that see nothing only, and rows of other sequences are untouched."""
+    hip = _hip()
+    n, scale = 150, D ** -0.5
+    table = hip.seq_table([n, 40])
+    q, k, v, do = (rnd(n + 40, D, dtype=dtype, seed=s) for s in range(4))
+    call = lambda q, k, v: (hip.attn_window_fwd(q, k, v, table, 1, 1, D, n, n, left=20, right=-3, sinks=2, lse=lse), lse)
+    lse = torch.zeros(n + 40, 1, device=DEV)
+    ok, ok_lse = (t.clone() for t in call(q, k, v))
+    i = torch.arange(n, device=DEV)
+    for name, at in (("q", 77), ("k", 90), ("k", 0)):
+        bad = {"q": q.clone(), "k": k.clone()}
+        bad[name][at, 5] = float("nan")
+        out, l = call(bad["q"], bad["k"], v)
+        sees = (i == at) if name == "q" else ((at >= i - 20) | (at < 2))       # no right edge
+        assert out[:n][sees].isnan().all() and l[:n, 0][sees].isnan().all()
+        assert torch.equal(out[n:], ok[n:]) and torch.equal(l[n:], ok_lse[n:])
+        assert torch.equal(out[:n][~sees], ok[:n][~sees]) and torch.equal(l[:n][~sees], ok_lse[:n][~sees])
+        g = hip.attn_window_bwd(bad["q"], bad["k"], v, out, l, do, table, 1, 1, D, n, n, left=20, right=-3, sinks=2)
+        assert g[0][:n][sees].isnan().all() and not any(t[n:].isnan().any() for t in g)
