@@ -1062,7 +1062,7 @@ def _ld(t):
 def rope_axes(x, pos, rope, heads, head_dim, out=None, inverse=False):
     """Rotary positions on x [M, heads * head_dim] (bf16 / fp16 / fp32; a column slice of packed q | k | v rows will do).
     pos: int32 [P, axes], M a multiple of P: row m stands at pos[m % P].  out: where to (x itself: in place; default: a new
-    tensor).  inverse: the turn back = the gradient's way."""
+    tensor).  inverse: the turn back = the gradient's way.  (No autograd: model.window_attention.rope_axes has it.)"""
     _need(x.dtype in _ELEMENTS, "rope_axes: x must be bf16, fp16 or fp32")
     _rows(x, heads * head_dim, x.dtype, x.device, "rope_axes: x")
     _need(pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape[1] == rope.axes and pos.is_contiguous() and pos.device == x.device,

@@ -41,3 +41,27 @@ def test_advance_refusals():
     for p, slots, text in ((past.long(), 8, "past must"), (past[:, None], 8, "past must"), (past, 0, "slots"), (past, 2 ** 31, "slots"), (past, 8, "no CPU path")):
         with pytest.raises(hip.OatError, match=text):
             hip.window_cache_advance(p, slots)
+
+
+def test_forward_mode_gradients_are_refused():
+    """The operators have gradients in reverse mode only: a tangent is refused, with and without a reverse-mode gradient beside it."""
+    from torch.autograd import forward_ad
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    seqs, rope, pos = hip.seq_table([4], device="cpu"), hip.RopeAxes((64,)), torch.zeros(4, 1, dtype=torch.int32)
+    cache = object.__new__(wa.WindowCache)                             # (the refusal comes before anything that needs a GPU)
+    cache.heads = cache.kv_heads = 1
+    cache.head_dim, cache.left, cache.sinks, cache.rope, cache.rolling = 64, 9, 0, None, True
+    cache.past = torch.zeros(4, dtype=torch.int32)
+    cache.k = cache.v = torch.zeros(4, 10, 1, 64, dtype=torch.bfloat16)
+    cache.pieces = torch.zeros(4)
+    for leaf in (torch.zeros(4, 192, dtype=torch.bfloat16), torch.zeros(4, 192, dtype=torch.bfloat16, requires_grad=True)):
+        calls = [lambda x: wa.window_attention(x, seqs, 1, 1, 64), lambda x: wa.window_attention(x, seqs, 1, 1, 64, rope=rope, pos=pos),
+                 lambda x: wa.rope_axes(x, pos, rope, 3, 64), lambda x: cache.step(x), lambda x: cache.prompt(x, seqs, 4)]
+        for call in calls:
+            with forward_ad.dual_level():
+                with pytest.raises(hip.OatError, match="forward mode"):
+                    call(forward_ad.make_dual(leaf, torch.ones_like(leaf)))
+                with pytest.raises(hip.OatError) as refused:           # no tangent: what is refused here is the missing GPU (or its buffers)
+                    call(leaf)
+                assert "forward mode" not in str(refused.value)
