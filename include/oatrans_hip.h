@@ -319,7 +319,7 @@ int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long l
 /* One new token of every sequence: qkv [B, (Hq + 2 Hkv) * D] (q | k | v); past[b] = tokens before it (< 0: takes no part: out is zero,
  * the cache stays; so does a plain cache without a slot left).  The query and key are turned by pos [B, n_axes] (rope NULL: not), the key
  * and value are written to their slot, and the query attends to what it sees.  Cache: cap slots; strides = 6 element strides {k: sequence, slot,
- * head; v: the same}, D contiguous.  Plain: token t in slot t, window `left` (< 0: none) and sinks as above.  Rolling: cap = sinks + left + 1
+ * head; v: the same}, D contiguous, no two places in one memory.  Plain: token t in slot t, window `left` (< 0: none) and sinks as above.  Rolling: cap = sinks + left + 1
  * slots, slot(t) = t < sinks ? t : sinks + (t - sinks) % (cap - sinks).  One launch.  workspace: exactly the bytes of its (B, Hq, Hkv, D)
  * and for these only, zero before the first use, left ready for the next call; calls that may run at the same time need one each. */
 size_t oat_attn_window_step_workspace_bytes(int B, int Hq, int Hkv, int D);

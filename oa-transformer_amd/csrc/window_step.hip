@@ -320,6 +320,23 @@ static int fail(const char* what, const char* why) {
   set_error(msg);
   return -2;
 }
+// whether two of the places {a sequence's, a slot's, a head's} of a cache overlap: by rising stride, each dimension has to step over all of
+// the smaller ones (a dimension of one takes no steps)
+static bool places_share(const long long* st, int B, int cap, int Hkv, int D) {
+  const int n[3] = {B, cap, Hkv};
+  long long extent = D;
+  bool done[3] = {n[0] <= 1, n[1] <= 1, n[2] <= 1};
+  for (int k = 0; k < 3; ++k) {
+    int least = -1;
+    for (int i = 0; i < 3; ++i)
+      if (!done[i] && (least < 0 || st[i] < st[least])) least = i;
+    if (least < 0) return false;
+    if (st[least] < extent) return true;
+    extent += st[least] * (n[least] - 1);
+    done[least] = true;
+  }
+  return false;
+}
 static const char* cache_wrong(const void* k, const void* v, const long long* st, int B, int cap, int Hkv, int D, int sinks) {
   if (D != 64 && D != 128) return "heads of 64 or 128 values";
   if (B < 0 || Hkv < 1 || cap < 1 || cap > (1 << 29) || sinks < 0 || sinks > (1 << 29)) return "no key heads, or a cache of no slots (or more than 2^29)";
@@ -349,6 +366,7 @@ extern "C" int oat_attn_window_step(const void* qkv, long long ldqkv, const int*
   if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
   if (dtype != 0 && dtype != 1) return fail(me, "element type: 0 (bf16) or 1 (fp16)");
   if (Hq < 1 || Hq % Hkv) return fail(me, "the query heads are not a multiple of the key heads");
+  if (places_share(strides, B, cap, Hkv, D) || places_share(strides + 3, B, cap, Hkv, D)) return fail(me, "slots of the cache share memory");
   if (!(scale > 0.f && scale < 1e30f)) return fail(me, "the scale is not a positive number");
   if (!qkv || !out || !past) return fail(me, "qkv, out and the counts of past tokens are needed");
   if (((uintptr_t)qkv | (uintptr_t)out) % 16 || ldqkv % 8 || ldo % 8 || ldqkv < (long long)(Hq + 2 * Hkv) * D || ldo < (long long)Hq * D)
@@ -398,6 +416,7 @@ static int cache_fill(const void* k, long long ldk, const void* v, long long ldv
   const char* me = "window_cache_fill";
   if (B == 0) return 0;
   if (const char* w = cache_wrong(kc, vc, strides, B, cap, Hkv, D, sinks)) return fail(me, w);
+  if (places_share(strides, B, cap, Hkv, D) || places_share(strides + 3, B, cap, Hkv, D)) return fail(me, "slots of the cache share memory");
   if (rows_k < 0 || max_k < 0 || B > 65535) return fail(me, "no rows, or more than 65535 sequences");
   if (rows_k == 0 || max_k == 0) return 0;
   if (!k || !v || !seqs || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)seqs) % 16 || ldk % 8 || ldv % 8 || ldk < (long long)Hkv * D || ldv < (long long)Hkv * D)

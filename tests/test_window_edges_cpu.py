@@ -65,3 +65,30 @@ def test_forward_mode_gradients_are_refused():
                 with pytest.raises(hip.OatError) as refused:           # no tangent: what is refused here is the missing GPU (or its buffers)
                     call(leaf)
                 assert "forward mode" not in str(refused.value)
+
+
+# ---------------------------------------------------------------------------------------------- caches whose slots share memory
+@pytest.mark.parametrize("k,v,ok", [
+    ((1024, 64, 64), (1024, 64, 64), False),                           # two heads in one place
+    ((0, 128, 64), (4096, 128, 64), False), ((4096, 128, 64), (0, 128, 64), False),     # one cache for all sequences (expand)
+    ((4096, 0, 64), (4096, 128, 64), False), ((1920, 128, 64), (2048, 128, 64), False), ((4096, 64, 128), (4096, 128, 64), False),
+    ((4096, 120, 64), (4096, 128, 64), False), ((4096, 128, 56), (4096, 128, 64), False),
+    ((2048, 128, 64), (2048, 128, 64), True), ((2048, 64, 1024), (2048, 128, 64), True), ((64, 256, 128), (128, 256, 64), True),
+    ((8192, 136, 72), (2048, 64, 1024), True)])
+def test_caches_whose_slots_share_memory_are_refused(k, v, ok):
+    """The step and the fill write the caches: no two slots (2 sequences, 16 slots, 2 heads of 64) may lie in one place."""
+    hip = _hip()
+    lib, st = hip.lib(), (LL * 6)(*k, *v)
+    # taken as far as the next refusal: the missing counts of the step, the misaligned rows of the fill
+    rc = lib.oat_attn_window_step(4096, 384, None, 4096, 4096, st, 16, 4096, 128, 2, 2, 2, 64, 0, -1, 0, 0, 0.125, None, None, 4096, 16, None)
+    _refused(hip, rc, b"needed" if ok else b"share")
+    _refused(hip, lib.oat_window_cache_fill(4097, 128, 4096, 128, 4096, 2, 10, 10, 4096, 4096, st, 16, 2, 64, 0, None), b"16-byte" if ok else b"share")
+
+
+def test_strides_of_a_single_sequence_slot_or_head_do_not_matter():
+    """torch gives a dimension of one any stride."""
+    hip = _hip()
+    for B, cap, Hkv, st in ((1, 16, 2, (0, 128, 64)), (2, 1, 2, (128, 0, 64)), (2, 16, 1, (1024, 64, 0)), (1, 1, 1, (0, 0, 0))):
+        rc = hip.lib().oat_attn_window_step(4096, 64 * 3 * Hkv, None, 4096, 4096, (LL * 6)(*st, *st), cap, 4096, 128, B, Hkv, Hkv, 64, 0, -1, 0, 0, 0.125,
+                                            None, None, 4096, 16, None)
+        _refused(hip, rc, b"needed")
