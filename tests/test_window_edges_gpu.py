@@ -119,3 +119,123 @@ def test_what_is_not_a_number_shows(D, dtype):
         assert torch.equal(out[:n][~sees], ok[:n][~sees]) and torch.equal(l[:n][~sees], ok_lse[:n][~sees])
         g = hip.attn_window_bwd(bad["q"], bad["k"], v, out, l, do, table, 1, 1, D, n, n, left=20, right=-3, sinks=2)
         assert g[0][:n][sees].isnan().all() and not any(t[n:].isnan().any() for t in g)
+
+
+# ---------------------------------------------------------------------------------------------- bounds that count every rounding once
+def tight(r, name, dtype, other):
+    """u |value| for its one rounding, u |term| for the 16-bit terms (worst case, or 6 deviations of independent ones; see
+    tests/test_window_gpu.py), 2^-14 of the terms for 32-bit sums, exponentials and the log-sum-exp.  What is below the type's normal
+    numbers is rounded to a multiple of its least one: off by half of that, s, for the result, and for every 16-bit probability or its
+    gradient s times what it multiplies - `other` is the sum of their sizes."""
+    u, s = half_step(dtype), torch.finfo(dtype).smallest_normal * half_step(dtype)
+    return u * r[name].abs() + torch.minimum(u * r[name + "_abs"], 6 * u * r[name + "_sq"]) + 2.0 ** -14 * r[name + "_abs"] + s + s * other
+
+
+def _check_attention(q, k, v, do, seqs, Hq, Hkv, D, left, right, sinks, scale):
+    """out, lse and the gradients of rows that all belong to a sequence, within `tight`"""
+    hip = _hip()
+    dtype = q.dtype
+    table = torch.tensor(seqs, dtype=torch.int32, device=DEV)
+    mq, mk, G = max(s[1] for s in seqs), max(s[3] for s in seqs), Hq // Hkv
+    lse = torch.empty(q.shape[0], Hq, device=DEV)
+    out = hip.attn_window_fwd(q, k, v, table, Hq, Hkv, D, mq, mk, left, right, sinks, scale, lse=lse)
+    dq, dk, dv = hip.attn_window_bwd(q, k, v, out, lse, do, table, Hq, Hkv, D, mq, mk, left, right, sinks, scale)
+    r = wo.attention(q, k, v, seqs, Hq, Hkv, D, left, right, sinks, scale, dout=do, out=out)
+    Q, K, V, dO = (t.double().abs() for t in (q, k, v, do))
+    seen_K, seen_V, seen_Q, seen_dO = torch.zeros_like(Q), torch.zeros_like(Q), torch.zeros_like(K), torch.zeros_like(K)
+    for q0, nq, k0, nk in seqs:
+        see = wo.visible(nq, nk, left, right, sinks, DEV).double()
+        for h in range(Hq):
+            a, b = slice(h * D, h * D + D), slice(h // G * D, h // G * D + D)
+            seen_K[q0:q0 + nq, a] = see @ K[k0:k0 + nk, b]
+            seen_V[q0:q0 + nq, a] = see @ V[k0:k0 + nk, b]
+            seen_Q[k0:k0 + nk, b] += see.t() @ Q[q0:q0 + nq, a]
+            seen_dO[k0:k0 + nk, b] += see.t() @ dO[q0:q0 + nq, a]
+    some = r["lse"] > -math.inf
+    within(lse[some], r["lse"][some], 2.0 ** -17 * (4 + r["lse"][some].abs()), "lse")
+    assert (lse[~some] == -math.inf).all()
+    # 1.01 *_off: delta from the rounded out, and 32-bit rounding of the terms that cancel in the probabilities' gradient
+    within(out, r["out"], tight(r, "out", dtype, seen_V), "out")
+    within(dq, r["dq"], tight(r, "dq", dtype, scale * seen_K) + 1.01 * r["dq_off"], "dq")
+    within(dk, r["dk"], tight(r, "dk", dtype, scale * seen_Q) + 1.01 * r["dk_off"], "dk")
+    within(dv, r["dv"], tight(r, "dv", dtype, seen_dO), "dv")
+    return r
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("lens,Hq,Hkv,D,left,right,sinks", [
+    ([2300], 1, 1, 64, 90, 0, 130), ([1100], 1, 1, 64, -1, -1, 0), ([1500], 1, 1, 64, 100, 0, 600), ([520, 130, 90], 2, 1, 128, 100, 30, 33),
+    ([700], 8, 1, 64, 64, 0, 2), ([1300, 700], 4, 1, 128, 100, 0, 40), ([1, 40, 1500], 2, 2, 128, -1, 0, 0)])
+def test_gradients_of_small_terms(lens, Hq, Hkv, D, left, right, sinks, dtype, size):
+    """Probabilities of a thousandth and less, and their gradients for a dout of 1 and 1 / 1000: in fp16 most of the terms are below its
+    normal numbers."""
+    M, starts = sum(lens), [sum(lens[:b]) for b in range(len(lens))]
+    seqs = [(a, n, a, n) for a, n in zip(starts, lens)]
+    q, k, v, do = rnd(M, Hq * D, dtype=dtype, seed=1), rnd(M, Hkv * D, dtype=dtype, seed=2), rnd(M, Hkv * D, dtype=dtype, seed=3), rnd(M, Hq * D, dtype=dtype, seed=4, scale=size)
+    _check_attention(q, k, v, do, seqs, Hq, Hkv, D, left, right, sinks, 0.9 / math.sqrt(D))
+
+
+# ---------------------------------------------------------------------------------------------- scores that grow along the keys
+def _moves(s, left, right, sinks):
+    """How often the forward kernel's reference score moves by a factor between 2^-40 and 1/2, by its rule on 64-bit scores of one head: the
+    maximum of the first 32 keys that a row sees, until 16 terms of a step (keys 8 (r >> 2) + 4 half + (r & 3) of it) sum to over 2^10 for
+    some row of 32."""
+    n = s.shape[0]
+    see = wo.visible(n, n, left, right, sinks)
+    keys = torch.tensor([[8 * (r >> 2) + 4 * half + (r & 3) for r in range(16)] for half in range(2)])
+    ref = torch.full((n,), -math.inf, dtype=torch.float64)
+    count = 0
+    for j in range(0, n, 32):
+        part = torch.full((n, 32), -math.inf, dtype=torch.float64)
+        part[:, :min(32, n - j)] = s[:, j:j + 32].masked_fill(~see[:, j:j + 32], -math.inf)
+        top = part.amax(1)
+        ref = torch.where((ref == -math.inf) & (top > -math.inf), top, ref)
+        term = torch.where(part > -math.inf, ((part - ref.clamp_min(-1e300)[:, None]) * math.log2(math.e)).clamp(max=1000).exp2(), torch.zeros_like(part))
+        over = (term[:, keys].sum(-1) > 1024).any(1)
+        for w in range(0, n, 32):
+            if over[w:w + 32].any():
+                new = torch.maximum(ref[w:w + 32], top[w:w + 32])
+                f = ((ref[w:w + 32] - new) * math.log2(math.e))
+                count += int(((f < -1) & (f > -40)).sum())
+                ref[w:w + 32] = new
+    return count
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,Hq,Hkv,D,left,right,sinks,slope,period,least", [
+    (300, 1, 1, 64, -1, 0, 0, 9.0, 300, 400), (300, 2, 1, 128, -1, -1, 0, 7.0, 300, 400), (700, 2, 2, 64, 120, 0, 0, 11.0, 170, 400),
+    (640, 4, 1, 128, 150, 0, 3, 10.0, 190, 400), (600, 2, 1, 64, 100, 20, 130, 8.0, 150, 400), (520, 1, 1, 128, 200, 60, 70, 6.0, 240, 300),
+    (450, 1, 1, 64, -1, 0, 200, 8.0, 200, 300)])
+def test_scores_that_grow_along_the_keys(n, Hq, Hkv, D, left, right, sinks, slope, period, least, dtype):
+    """Scores that rise by 6 to 11 (natural units) per 64 keys, in a saw: the reference of a row moves, by factors that leave weight to what
+    came before, more than once in many rows - behind sinks, at masked edges, in rows that begin later than their neighbours."""
+    scale = D ** -0.5
+    j = torch.arange(n, dtype=torch.float64)
+    rise = slope * (j % period) / 64
+    # q and k share a direction of sixteen values: 2 * rise / 2 / (16 * scale) * 16 * scale = rise, on top of noise
+    q, k, v, do = (rnd(n, h * D, dtype=dtype, seed=s, scale=0.5) for s, h in ((1, Hq), (2, Hkv), (3, Hkv), (4, Hq)))
+    q.view(n, Hq, D)[..., :16] = 1.0
+    k.view(n, Hkv, D)[..., :16] = (rise / (16 * scale)).to(dtype).to(DEV)[:, None, None]
+    moved = sum(_moves((q.view(n, Hq, D)[:, h].double() @ k.view(n, Hkv, D)[:, h // (Hq // Hkv)].double().t() * scale).cpu(), left, right, sinks)
+                for h in range(Hq))
+    assert moved >= least, moved
+    r = _check_attention(q, k, v, do, [(0, n, 0, n)], Hq, Hkv, D, left, right, sinks, scale)
+    assert r["lse"].max() > 15
+
+
+def test_step_shows_what_is_not_a_number():
+    """A query, or a key in the cache, that is not a number: in one piece and in many."""
+    hip = _hip()
+    for cap, at in ((300, 17), (5000, 4100), (5000, 3)):
+        kc, vc, x = rnd(2, cap, 1, 64, seed=1), rnd(2, cap, 1, 64, seed=2), rnd(2, 192, seed=3)
+        past = torch.full((2,), cap - 1, dtype=torch.int32, device=DEV)
+        ok = hip.attn_window_step(x, past, kc, vc, 1)
+        bad = kc.clone()
+        bad[0, at, 0, 9] = float("nan")
+        out = hip.attn_window_step(x, past, bad, vc, 1)
+        assert out[0].isnan().all() and torch.equal(out[1], ok[1])
+        y = x.clone()
+        y[1, 3] = float("nan")
+        out = hip.attn_window_step(y, past, kc, vc, 1)
+        assert out[1].isnan().all() and torch.equal(out[0], ok[0])
