@@ -158,6 +158,8 @@ class WindowCache:
     def __init__(self, B, heads, kv_heads, head_dim, window=None, sinks=0, slots=None, rope=None, dtype=torch.bfloat16, device="cuda"):
         if (window is None) == (slots is None) or (window is not None and window < 1) or (slots is not None and slots < 1):
             raise hip.OatError("WindowCache: either a window (it rolls) or a number of slots, at least 1")
+        if head_dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads or dtype not in (torch.bfloat16, torch.float16) or B < 0 or sinks < 0:
+            raise hip.OatError("WindowCache: heads of 64 or 128 in bf16 or fp16, query heads a multiple of the key heads, no negative sinks")
         self.rolling, self.left = window is not None, -1 if window is None else window - 1
         self.slots = slots if window is None else sinks + window
         self.heads, self.kv_heads, self.head_dim, self.sinks, self.rope = heads, kv_heads, head_dim, sinks, rope

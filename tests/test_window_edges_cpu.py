@@ -92,3 +92,101 @@ def test_strides_of_a_single_sequence_slot_or_head_do_not_matter():
         rc = hip.lib().oat_attn_window_step(4096, 64 * 3 * Hkv, None, 4096, 4096, (LL * 6)(*st, *st), cap, 4096, 128, B, Hkv, Hkv, 64, 0, -1, 0, 0, 0.125,
                                             None, None, 4096, 16, None)
         _refused(hip, rc, b"needed")
+
+
+# ---------------------------------------------------------------------------------------------- what the binding checks, by message
+def _calls():
+    """(what it is, call, message): CPU tensors throughout, so a check that is not made ends in 'no CPU path' instead of its own message"""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    BF, i32 = torch.bfloat16, torch.int32
+    rope = hip.RopeAxes((16, 24, 24))
+    x, pos = torch.zeros(4, 64), torch.zeros(4, 3, dtype=i32)
+    R = lambda **c: (lambda a: hip.rope_axes(a["x"], a["pos"], rope, a["heads"], a["dim"], out=a["out"]))({**dict(x=x, pos=pos, heads=1, dim=64, out=None), **c})
+    yield "rope", lambda: R(), "no CPU path"
+    yield "rope: 64-bit x", lambda: R(x=x.double()), "must be bf16, fp16 or fp32"
+    yield "rope: x of one dimension", lambda: R(x=x[0]), "rope_axes: x: need"
+    yield "rope: narrow x", lambda: R(heads=2), "rope_axes: x: need"
+    yield "rope: stepped columns", lambda: R(x=x[:, ::2], dim=32), "rope_axes: x: need"
+    yield "rope: 64-bit pos", lambda: R(pos=pos.long()), "pos must be"
+    yield "rope: two axes", lambda: R(pos=pos[:, :2]), "pos must be"
+    yield "rope: pos not contiguous", lambda: R(pos=torch.zeros(4, 6, dtype=i32)[:, ::2]), "pos must be"
+    yield "rope: pos elsewhere", lambda: R(pos=pos.to("meta")), "pos must be"
+    yield "rope: short out", lambda: R(out=torch.zeros(3, 64)), "number of rows"
+    yield "rope: out of another type", lambda: R(out=torch.zeros(4, 64, dtype=BF)), "rope_axes: out: need"
+    yield "rope layer: width", lambda: wa.rope_axes(x, pos, rope, 2, 64), r"\[M, heads \* head_dim\]"
+    b, seqs = torch.zeros(4, 64, dtype=BF), hip.seq_table([4], device="cpu")
+    lse = torch.zeros(4, 1)
+    base = dict(q=b, k=b, v=b, seqs=seqs, heads=1, kv=1, D=64, mq=4, mk=4)
+    F = lambda out=None, lse=None, **c: (lambda a: hip.attn_window_fwd(*a.values(), out=out, lse=lse))({**base, **c})
+    yield "forward", lambda: F(), "no CPU path"
+    for name, change, text in (("32 bits", dict(q=x, k=x, v=x), "bf16 or fp16"), ("narrow q", dict(heads=2), "attn_window_fwd: q: need"), ("narrow k", dict(kv=2), "attn_window_fwd: k: need"),
+                               ("k of another type", dict(k=b.half()), "attn_window_fwd: k: need"), ("v of another type", dict(v=b.half()), "attn_window_fwd: v: need"),
+                               ("v elsewhere", dict(v=b.to("meta")), "attn_window_fwd: v: need"), ("stepped q", dict(q=torch.zeros(4, 128, dtype=BF)[:, ::2]), "attn_window_fwd: q: need"),
+                               ("rows of k", dict(k=b[:3]), "different numbers of rows"), ("rows of v", dict(v=b[:3]), "different numbers of rows"), ("64-bit seqs", dict(seqs=seqs.long()), "seqs must be"),
+                               ("seqs of three", dict(seqs=seqs[:, :3].contiguous()), "seqs must be"), ("seqs not contiguous", dict(seqs=torch.zeros(1, 8, dtype=i32)[:, ::2]), "seqs must be"),
+                               ("seqs elsewhere", dict(seqs=seqs.to("meta")), "seqs must be"), ("negative count", dict(mq=-1), "largest counts"), ("large count", dict(mk=2 ** 29 + 1), "largest counts")):
+        yield "forward: " + name, lambda change=change: F(**change), text
+    yield "forward: lse's shape", lambda: F(lse=torch.zeros(4, 2)), "lse must be"
+    yield "forward: lse's type", lambda: F(lse=lse.double()), "lse must be"
+    yield "forward: lse's order", lambda: hip.attn_window_fwd(torch.zeros(4, 128, dtype=BF), b, b, seqs, 2, 1, 64, 4, 4, lse=torch.zeros(2, 4).t()), "lse must be"
+    yield "forward: short out", lambda: F(out=b[:3]), "number of rows than q"
+    yield "forward: out's type", lambda: F(out=x), "attn_window_fwd: out: need"
+    G = lambda **c: (lambda a: hip.attn_window_bwd(a["q"], a["k"], a["v"], a["out"], a["lse"], a["dout"], seqs, 1, 1, 64, 4, 4, dq=a["dq"], dk=a["dk"], dv=a["dv"], workspace=a["ws"]))(
+        {**base, **dict(out=b, lse=lse, dout=b, dq=None, dk=None, dv=None, ws=None), **c})
+    yield "backward", lambda: G(), "no CPU path"
+    for name, change, text in (("out's type", dict(out=x), "attn_window_bwd: out: need"), ("dout's type", dict(dout=x), "attn_window_bwd: dout: need"), ("short dout", dict(dout=b[:3]), "as many rows as q"),
+                               ("short out", dict(out=b[:3]), "as many rows as q"), ("lse's shape", dict(lse=torch.zeros(4, 2)), "lse must be"), ("dq's type", dict(dq=x), "attn_window_bwd: dq: need"),
+                               ("narrow dk", dict(dk=b[:, :32]), "attn_window_bwd: dk: need"), ("dv elsewhere", dict(dv=b.to("meta")), "attn_window_bwd: dv: need"), ("short dq", dict(dq=b[:3]), "as many rows as q, k, v"),
+                               ("short dv", dict(dv=b[:3]), "as many rows as q, k, v"), ("workspace elsewhere", dict(ws=lse.to("meta")), "workspace must be"),
+                               ("stepped workspace", dict(ws=torch.zeros(64)[::2]), "workspace must be")):
+        yield "backward: " + name, lambda change=change: G(**change), text
+    c, past, row, ws = torch.zeros(4, 8, 1, 64, dtype=BF), torch.zeros(4, dtype=i32), torch.zeros(4, 192, dtype=BF), torch.zeros(4)
+    S = lambda **o: (lambda a: hip.attn_window_step(a["qkv"], a["past"], a["k"], a["v"], a["heads"], rope=a["rope"], pos=a["pos"], pieces=a["ws"], out=a["out"]))(
+        {**dict(qkv=row, past=past, k=c, v=c, heads=1, rope=None, pos=None, ws=ws, out=None), **o})
+    yield "step", lambda: S(), "no CPU path"
+    for name, change, text in (("64-bit past", dict(past=past.long()), "past must be"), ("short past", dict(past=past[:3]), "past must be"), ("past elsewhere", dict(past=past.to("meta")), "past must be"),
+                               ("stepped past", dict(past=torch.zeros(8, dtype=i32)[::2]), "past must be"), ("short qkv", dict(qkv=row[:3]), "one row of qkv"), ("narrow qkv", dict(heads=2), "attn_window_step: qkv: need"),
+                               ("qkv's type", dict(qkv=row.half()), "differ in type or device"), ("qkv elsewhere", dict(qkv=row.to("meta")), "differ in type or device"), ("caches that differ", dict(v=c[:, :4]), "both alike"),
+                               ("32-bit caches", dict(k=c.float(), v=c.float()), "both alike"), ("caches of three dimensions", dict(k=c[0], v=c[0]), "both alike"), ("stepped caches", dict(k=c[..., ::2], v=c[..., ::2]), "both alike"),
+                               ("no pos", dict(rope=rope), "pos must be"), ("short pos", dict(rope=rope, pos=pos[:3]), "pos must be"), ("64-bit pos", dict(rope=rope, pos=pos.long()), "pos must be"),
+                               ("stepped workspace", dict(ws=torch.zeros(64)[::2]), "pieces must be"), ("short out", dict(out=b[:3]), "one row of out"), ("out's type", dict(out=x), "attn_window_step: out: need")):
+        yield "step: " + name, lambda change=change: S(**change), text
+    seqs4 = hip.seq_table([1, 1, 1, 1], device="cpu")
+    L = lambda **o: (lambda a: hip.window_cache_fill(a["k"], a["v"], a["seqs"], a["kc"], a["vc"], a["most"]))({**dict(k=b, v=b, seqs=seqs4, kc=c, vc=c, most=4), **o})
+    yield "fill", lambda: L(), "no CPU path"
+    for name, change, text in (("B", dict(seqs=seqs), "seqs must be"), ("64-bit seqs", dict(seqs=seqs4.long()), "seqs must be"), ("k's type", dict(k=b.half()), "window_cache_fill: k: need"),
+                               ("narrow v", dict(v=b[:, :32]), "window_cache_fill: v: need"), ("rows", dict(v=b[:3]), "different numbers"), ("count", dict(most=-1), "largest count"), ("large count", dict(most=2 ** 30), "largest count")):
+        yield "fill: " + name, lambda change=change: L(**change), text
+    W = lambda **o: (lambda a: wa.window_attention(a.pop("qkv"), a.pop("seqs"), a.pop("heads"), a.pop("kv"), a.pop("D"), **a))({**dict(qkv=row, seqs=seqs, heads=1, kv=1, D=64), **o})
+    yield "layer", lambda: W(), "no CPU path"
+    yield "layer: gradient", lambda: W(qkv=row.clone().requires_grad_()), "no CPU path"
+    for name, change, text in (("width", dict(D=128), r"qkv must be \[M, 384\]"), ("32 bits", dict(qkv=row.float()), "bf16 or fp16"), ("stepped columns", dict(qkv=torch.zeros(4, 384, dtype=BF)[:, ::2]), "unit column stride"),
+                               ("rope alone", dict(rope=rope), "belong together"), ("pos alone", dict(pos=pos), "belong together"), ("64-bit pos", dict(rope=rope, pos=pos.long()), "pos must be"),
+                               ("64-bit seqs", dict(seqs=seqs.long()), "seqs must be"), ("right with a cache", dict(right=1, cache=(c[:1], c[:1])), "causal attention"),
+                               ("few slots", dict(longest=9, qkv=torch.zeros(9, 192, dtype=BF), cache=(c[:1], c[:1])), "slot for every token"),
+                               ("gradient with a cache", dict(qkv=row.clone().requires_grad_(), cache=(c[:1], c[:1])), "without a gradient"), ("cache of another batch", dict(cache=(c, c)), r"caches must be \[1, slots"),
+                               ("cache's type", dict(cache=(c[:1].half(), c[:1].half())), "caches must be"), ("caches that differ", dict(cache=(c[:1], c[:1, :4])), "both alike")):
+        yield "layer: " + name, lambda change=change: W(**change), text
+    yield "cache: window and slots", lambda: wa.WindowCache(1, 1, 1, 64, window=4, slots=4, device="cpu"), "either a window"
+    yield "cache: neither", lambda: wa.WindowCache(1, 1, 1, 64, device="cpu"), "either a window"
+    yield "cache: no window", lambda: wa.WindowCache(1, 1, 1, 64, window=0, device="cpu"), "either a window"
+    yield "cache: no slots", lambda: wa.WindowCache(1, 1, 1, 64, slots=0, device="cpu"), "either a window"
+    yield "cache: sinks", lambda: wa.WindowCache(1, 1, 1, 64, window=4, sinks=-1, device="cpu"), "sinks"
+    yield "cache: heads", lambda: wa.WindowCache(1, 3, 2, 64, window=4, device="cpu"), "multiple"
+    yield "cache: head_dim", lambda: wa.WindowCache(1, 2, 2, 32, window=4, device="cpu"), "64 or 128"
+    yield "cache: type", lambda: wa.WindowCache(1, 2, 2, 64, window=4, dtype=torch.float32, device="cpu"), "bf16 or fp16"
+    yield "table: lengths", lambda: hip.seq_table([1, 2], [1]), "one count"
+    yield "table: negative", lambda: hip.seq_table([1, -1]), "one count"
+    yield "table: rows", lambda: hip.seq_table([1, 2], q_rows=(0,)), "first row"
+
+
+def test_every_check_of_the_binding_says_what_is_wrong():
+    hip = _hip()
+    count = 0
+    for name, call, text in _calls():
+        with pytest.raises(hip.OatError, match=text):
+            call()
+            pytest.fail(f"{name}: taken")
+        count += 1
+    assert count > 90
