@@ -311,7 +311,9 @@ int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long l
                         float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
                         int left, int right, int sinks, float scale, void* stream);
 size_t oat_attn_window_bwd_workspace_bytes(int rows_q, int B, int max_q, int max_k, int Hq, int Hkv, int D, int left, int sinks);
-/* dq, dk, dv of the same call (written, not accumulated; fixed order of every sum).  Sequences must not share query or key rows. */
+/* dq, dk, dv of the same call (written, not accumulated; fixed order of every sum).  Sequences must not share query or key rows.
+ * The matrix unit takes the probabilities' gradient dS = P (dout . v - delta), before the scale, in the rows' type.  fp16: a |dS| of 65520
+ * or more gives inf or nan in its query's dq and its key's dk (never a wrong number), one below 2^-14 is held in steps of 2^-24. */
 int oat_attn_window_bwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* out, long long ldo,
                         const float* lse, const void* dout, long long lddo, void* dq, long long lddq, void* dk, long long lddk, void* dv,
                         long long lddv, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,

@@ -124,7 +124,8 @@ def window_attention(qkv, seqs, heads, kv_heads, head_dim, left=-1, right=0, sin
     rope, pos: rotary positions of q and k, pos int32 [P, axes] with M a multiple of P.
     packed: the caller states that every row belongs to a sequence; otherwise rows of none (padding) get zeros, and zero gradients.
     Rows of no sequence may hold anything; rows of a sequence have to be finite (a masked pair's weight is an exact zero, and it is
-    multiplied).
+    multiplied).  fp16 gradients: the probabilities' gradient P (dout . v - delta) has to stay below 65504: beyond, dq and dk are inf or nan,
+    which a loss scaler sees; below 2^-14 it loses bits.
     cache: (k, v) of [B, slots, kv_heads, head_dim] that take the prompt's turned keys and its values (no gradient then); fewer slots
     than tokens only where they are the sinks and the window, sinks + left + 1."""
     D = head_dim

@@ -154,11 +154,19 @@ def _check_attention(q, k, v, do, seqs, Hq, Hkv, D, left, right, sinks, scale):
     some = r["lse"] > -math.inf
     within(lse[some], r["lse"][some], 2.0 ** -17 * (4 + r["lse"][some].abs()), "lse")
     assert (lse[~some] == -math.inf).all()
+    # (what is beyond the type's largest number by more than its tolerance is inf of its sign)
+    top = torch.finfo(dtype).max
+
+    def within_type(got, ref, tol, what):
+        inf = ref.abs() - tol > top
+        assert (got[inf].double() == ref[inf].sign() * math.inf).all(), what
+        near = ~inf & (ref.abs() + tol >= top)
+        within(got[~inf & ~near], ref[~inf & ~near], tol[~inf & ~near], what)
     # 1.01 *_off: delta from the rounded out, and 32-bit rounding of the terms that cancel in the probabilities' gradient
-    within(out, r["out"], tight(r, "out", dtype, seen_V), "out")
-    within(dq, r["dq"], tight(r, "dq", dtype, scale * seen_K) + 1.01 * r["dq_off"], "dq")
-    within(dk, r["dk"], tight(r, "dk", dtype, scale * seen_Q) + 1.01 * r["dk_off"], "dk")
-    within(dv, r["dv"], tight(r, "dv", dtype, seen_dO), "dv")
+    within_type(out, r["out"], tight(r, "out", dtype, seen_V), "out")
+    within_type(dq, r["dq"], tight(r, "dq", dtype, scale * seen_K) + 1.01 * r["dq_off"], "dq")
+    within_type(dk, r["dk"], tight(r, "dk", dtype, scale * seen_Q) + 1.01 * r["dk_off"], "dk")
+    within_type(dv, r["dv"], tight(r, "dv", dtype, seen_dO), "dv")
     return r
 
 
@@ -239,3 +247,44 @@ def test_step_shows_what_is_not_a_number():
         y[1, 3] = float("nan")
         out = hip.attn_window_step(y, past, kc, vc, 1)
         assert out[1].isnan().all() and torch.equal(out[0], ok[0])
+
+
+# ---------------------------------------------------------------------------------------------- the upper end of fp16
+@pytest.mark.parametrize("D,Hq,Hkv,n,sinks", [(64, 2, 1, 300, 0), (128, 2, 2, 300, 0), (64, 1, 1, 1500, 2), (128, 4, 2, 1500, 2)])
+def test_fp16_gradients_up_to_the_limit_and_beyond(D, Hq, Hkv, n, sinks):
+    """Up to |dS| = 6e4 the gradients are right; beyond 65520 the query's dq and the key's dk are inf or nan, everything else is what it is
+    without that term's row."""
+    hip = _hip()
+    scale = D ** -0.5
+    q, k, v = rnd(n, Hq * D, dtype=HF, seed=1, scale=0.25), rnd(n, Hkv * D, dtype=HF, seed=2, scale=0.25), rnd(n, Hkv * D, dtype=HF, seed=3, scale=2.0)
+    do = rnd(n, Hq * D, dtype=HF, seed=4)
+    seqs = [(0, n, 0, n)]
+
+    def terms_of_scores():
+        Q, K, V, O = (t.double().view(n, -1, D).transpose(0, 1) for t in (q, k.repeat(1, 1), v, do))
+        K, V = (t.repeat_interleave(Hq // Hkv, 0) for t in (K, V))
+        see = wo.visible(n, n, 2, 0, sinks, DEV)
+        P = torch.softmax((Q @ K.transpose(1, 2).contiguous() * scale).masked_fill(~see, -math.inf), 2)
+        dP = O @ V.transpose(1, 2).contiguous()
+        return P * (dP - (P * dP).sum(2, keepdim=True))
+    top = terms_of_scores().abs().max().item()
+    do = (do.double() * (6.0e4 / top)).to(HF)
+    assert do.isfinite().all() and 5.5e4 < terms_of_scores().abs().max().item() < 6.4e4
+    _check_attention(q, k, v, do, seqs, Hq, Hkv, D, 2, 0, sinks, scale)
+    # one query's gradient times four
+    table, at = hip.seq_table([n]), int(terms_of_scores().abs().amax(2)[0].argmax())
+    lse = torch.empty(n, Hq, device=DEV)
+    out = hip.attn_window_fwd(q, k, v, table, Hq, Hkv, D, n, n, 2, 0, sinks, scale, lse=lse)
+    ok = hip.attn_window_bwd(q, k, v, out, lse, do, table, Hq, Hkv, D, n, n, 2, 0, sinks, scale)
+    do[at, :D] = (do[at, :D].double() * 4).clamp(-6.5e4, 6.5e4).to(HF)
+    over = terms_of_scores().abs() > 65520                              # [Hq, n, n]
+    got = hip.attn_window_bwd(q, k, v, out, lse, do, table, Hq, Hkv, D, n, n, 2, 0, sinks, scale)
+    rows = over.any(2).t().repeat_interleave(D, 1)
+    keys = over.view(Hkv, -1, n, n).any(1).any(1).t().repeat_interleave(D, 1)
+    assert over.any() and not got[0][rows].isfinite().any() and not got[1][keys].isfinite().any()
+    far = torch.ones(n, dtype=torch.bool, device=DEV)                    # keys that the query does not see
+    far[:sinks], far[at - 2:at + 1] = False, False
+    assert torch.equal(got[2][far], ok[2][far]) and got[0][~rows].isfinite().all() and got[1][~keys & far[:, None]].isfinite().all()
+    other = torch.ones(n, dtype=torch.bool, device=DEV)
+    other[at] = False
+    assert torch.equal(got[0][other], ok[0][other])
