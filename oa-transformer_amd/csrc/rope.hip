@@ -6,7 +6,9 @@
 //
 // Bound: every element is read and written once - HBM.  The angles are formed once per row and pair (64-bit product, one sincospi),
 // kept in the LDS and used by all heads of the row: 1 / (2 * heads) of an angle per element.  A workgroup takes ROWS rows so that
-// each thread forms about one angle; then 16-byte loads of u and v chunks, one store each.
+// each thread forms about one angle; then 16-byte loads of u and v chunks, one store each.  Plain stores: the attention reads the output
+// next.  (Past the caches where they are over 96 MB, a call among calls takes 64 us instead of 67 - 32 clips of 1569 tokens, 308 MB - or 70
+// instead of 72 - the 32-bit gradient of four 16-frame clips - but the layer on those 32 clips 249 us instead of 241, on 64 equal.)
 #include "rope.h"
 
 namespace oat {
@@ -21,18 +23,9 @@ struct RopeArgs {
   OatRope rope;
 };
 
-// FAR: the stores bypass the caches, for outputs that are larger than these would keep for the next reader.  On 154 MB out of 230 MB rows
-// (bf16, 32 clips of 1569 tokens, 24 heads of 64): 54 us = 5.7 TB/s read and written against 62 us with plain stores; on 43 MB, which the
-// next kernel finds in the caches, plain stores are faster (15.2 against 16.4 us).  (A copy of 256 MB runs at 5.4 TB/s.)
-template <bool FAR, class V> OAT_DEV void store(void* p, V v) {
-  if constexpr (FAR) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
-  else *reinterpret_cast<V*>(p) = v;
-}
-constexpr long long FAR_BYTES = 96ll << 20;
-
 // VEC: every chunk of 16 bytes of u has its partners in one chunk of v (or, interleaved, in itself) and all addresses are multiples
 // of 16 bytes; otherwise element by element.
-template <class T, bool VEC, bool FAR>
+template <class T, bool VEC>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
   __shared__ float2 cs[1024];                        // rows * n_pairs <= 1024
   constexpr int N = Elem<T>::N;
@@ -58,7 +51,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
       T* po = a.out + (size_t)(m0 + r) * a.ldo + h * a.dim;
       const float2* w = cs + r * np;
       if (c >= turn) {
-        store<FAR>(po + R + (c - turn) * N, *reinterpret_cast<const V*>(px + R + (c - turn) * N));
+        *reinterpret_cast<V*>(po + R + (c - turn) * N) = *reinterpret_cast<const V*>(px + R + (c - turn) * N);
       } else if (a.rope.interleaved) {
         V x = *reinterpret_cast<const V*>(px + c * N);
 #pragma unroll
@@ -67,7 +60,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
           x[2 * e] = (T)y.x;
           x[2 * e + 1] = (T)y.y;
         }
-        store<FAR>(po + c * N, x);
+        *reinterpret_cast<V*>(po + c * N) = x;
       } else {
         V xu = *reinterpret_cast<const V*>(px + c * N), xv = *reinterpret_cast<const V*>(px + np + c * N);
 #pragma unroll
@@ -76,8 +69,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs<T> a) {
           xu[e] = (T)y.x;
           xv[e] = (T)y.y;
         }
-        store<FAR>(po + c * N, xu);
-        store<FAR>(po + np + c * N, xv);
+        *reinterpret_cast<V*>(po + c * N) = xu;
+        *reinterpret_cast<V*>(po + np + c * N) = xv;
       }
     }
   } else {
@@ -112,10 +105,8 @@ static int rope_run(const void* x, long long ldx, void* out, long long ldo, cons
                    ((uintptr_t)x | (uintptr_t)out) % 16 == 0;
   const int blocks = (int)(((long long)M + a.rows - 1) / a.rows);
   if (blocks >= 1 << 23) { set_error("rope_axes: more rows than a launch can hold (2^23 workgroups)"); return -2; }
-  const bool far = (long long)M * heads * dim * (long long)sizeof(T) > FAR_BYTES;
-  if (vec && far) OAT_LAUNCH((rope_kernel<T, true, true>), dim3(blocks), dim3(256), 0, s, a);
-  else if (vec) OAT_LAUNCH((rope_kernel<T, true, false>), dim3(blocks), dim3(256), 0, s, a);
-  else OAT_LAUNCH((rope_kernel<T, false, false>), dim3(blocks), dim3(256), 0, s, a);
+  if (vec) OAT_LAUNCH((rope_kernel<T, true>), dim3(blocks), dim3(256), 0, s, a);
+  else OAT_LAUNCH((rope_kernel<T, false>), dim3(blocks), dim3(256), 0, s, a);
   return check_launch("rope_axes");
 }
 
