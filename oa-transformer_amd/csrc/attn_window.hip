@@ -8,11 +8,17 @@ namespace oat {
 //     S^T = K Q^T      P^T = exp2(c S^T - c m)      O^T += V^T P^T       c = scale log2(e), m = running maximum of the row
 // The query is the COLUMN of S^T: a lane holds 16 of 32 keys of ONE query, so maximum and sum of a row are register work and one
 // exchange with lane ^ 32, and P^T is the B operand of the second product where it stands.
-// Bound: instruction issue.  The 32 keys of a step are 8 matrix instructions (heads of 64) and about 130 vector ones; two waves of a SIMD
-// take 293 clocks for the first alone, 313 for the second alone, 440 for both: the two units overlap for a third of it.  128 queries
-// share each staged tile, so the LDS and HBM are idle most of the time.  Measured: two clips of 7057 tokens (12 heads of 64, window of
-// 882 to each side) 108 us = 665 TFLOP/s; 8191 tokens (32 / 8 heads of 128, causal, window of 1024) 174 us = 743; six packed texts of
-// 512 to 2048 (16 / 4 heads of 128, window of 512) 66 us = 418: a fourth of the products there are masked at the window's edges.
+// Bound: no unit alone, but the way in which two or three waves of a SIMD share them.  Two clips of 7057 tokens (12 heads of 64, window of
+// 882 to each side), by counters: the matrix unit is busy 37 % of the time (8 products of 32 clocks per 32 keys of a wave), the vector unit
+// 57 % (75 instructions, 16 of them exponentials), the LDS 18 % (4 clocks a KB, no bank conflicts); 2.3 waves are on a SIMD (the registers
+// allow 3, the list of tiles is 1.75 rounds of that), and of their time they issue in 42 %, wait to issue in 32 % and for data or the
+// barrier in 26 %.  Per 32 keys of a wave that is 700 clocks; in a loop of nothing else the same products take 295, the exponentials, sums
+// and conversions 310, both 420 to 440.  Heads of 128 (8191 tokens below): matrix unit 42 %, vector unit 38 %, 1.8 waves.
+// Measured (median of 60 runs): the clips 109 us = 660 TFLOP/s; 8191 tokens (32 / 8 heads of 128, causal, window of 1024) 187 us = 691; six
+// packed texts of 512 to 2048 (16 / 4 heads of 128, window of 512) 63 us = 435: a fourth of the products there are masked at the window's
+// edges, and 1.5 waves are on a SIMD.
+// Roundings: P to the operands' 16 bits (pack8); its sum l is of the terms before that, in 32 bits - the terms are off by half a step at most,
+// up and down alike.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
@@ -234,9 +240,10 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinArgs a) {
 // Two kernels that form S and dO V^T again, one over queries (dQ), one over keys (dK, dV; the query heads that share a key head are
 // summed in the workgroup): 7 products for the 5 of one kernel with atomic sums, but every sum has one fixed order.
 
-// dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  Bound: instruction issue, as above, with three products
-// for one exponential: the clips of above 139 us = 775 TFLOP/s, the packed texts 80 us = 517 (141 and 87 with the
-// turn back).
+// dQ and delta: the forward's walk, S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  Bound: as above, with three products
+// for one exponential (matrix unit 44 % of the time, vector unit 53 %, LDS 22 %): the clips of above 142 us = 758 TFLOP/s, the packed texts
+// 86 us = 480 (with the turn back, which takes 2 and 7 of these).  delta is formed from the forward's rounded out, half a step off at most,
+// so that the forward need not leave 32-bit rows.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(WinArgs a) {
   constexpr int TB = TILE * D * 2;
@@ -460,8 +467,8 @@ template <int D> OAT_DEV void clear_keys(const WinArgs& a, const Place& pl, int 
 }
 
 // 128 keys, 32 a wave: S = Q K^T, dP = dO V^T with the key as the column, dV^T += dO^T P, dK^T += Q^T dS; queries and their gradients
-// pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: instruction issue (four products for one exponential): the
-// clips of above 180 us = 797 TFLOP/s.
+// pass through the LDS in tiles of 64, with their lse2 and delta.  Bound: as above (four products for one exponential; matrix unit
+// 43 % of the time, vector unit 48 %, LDS 33 %): the clips of above 182 us = 788 TFLOP/s.
 template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;
@@ -578,8 +585,8 @@ template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) 
 
 // The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other
 // through the LDS, and then one adds up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum
-// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above: 111 us = 497 TFLOP/s
-// (115 with the sinks' far queries, 121 with the turn back too).
+// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above, with the sinks' far queries and the turn
+// back: 113 us = 488 TFLOP/s (matrix unit 29 %, vector unit 24 %, 1.4 waves on a SIMD).
 template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, char* lds) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;

@@ -48,9 +48,10 @@ template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
 // next keys while it works on these): 64 KB in flight per CU, with 64 KB of LDS a workgroup (D = 128), so that two or more share a CU.  S^T = K Q^T and
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
 // The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
-// new token writes its row to the cache first.  Pieces are joined by the workgroup that finishes last, in a fixed order.
-// Measured: 64 sequences of up to 4096 tokens, 32 / 8 heads of 128: 576 MB in 114 us = 5.0 TB/s; two of 65536 visible tokens: 537 MB in
-// 104 us = 5.1 (a large copy: 4.9 to 5.4); one of 512, 12 heads of 64: 7.7 us, a chain of dependent loads.
+// new token writes its row to the cache first.  The turned query and key and the probabilities are rounded to the operands' 16 bits (the
+// cache holds no more, the matrix unit takes no more); scores, statistics and sums are 32-bit.  Pieces are joined by the workgroup that finishes last, in a fixed order.
+// Measured: 64 sequences of up to 4096 tokens, 32 / 8 heads of 128: 576 MB in 117 us = 4.9 TB/s; two of 65536 visible tokens: 537 MB in
+// 107 us = 5.0 (a large copy: 4.9 to 5.4); one of 512, 12 heads of 64: 7.8 us, a chain of dependent loads.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void win_step_kernel(StepArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -472,9 +473,11 @@ extern "C" int oat_window_cache_advance(int* past, int B, int cap, void* stream)
   return check_launch(me);
 }
 
-// ---- what a layer on packed q | k | v rows does, in one call each way (one crossing into the library instead of three)
-// whether the gradient's way back through the rotary positions can be taken where dq and dk are formed: a pair's two values have to
-// meet in one lane, as those of a head's two halves do
+// ---- what a layer on packed q | k | v rows does, in one call each way (one crossing into the library instead of three).  The turned q and k
+// are held in the rows' type: the matrix unit takes no more, and the cache keeps the keys as they are
+// whether the gradient's way back through the rotary positions is taken where dq and dk are formed.  A pair's two values have to meet in one
+// lane: those of a head's two halves do, in one register of two fragments, and this is the ladder that has the code.  (So would neighbours,
+// and halves of fewer pairs that are a multiple of 8: such ladders take a pass of their own and round twice.)
 static bool turns_in_halves(const OatRope* rope, int D) { return !rope->interleaved && 2 * rope->n_pairs == D; }
 static int packed_wrong(const char* me, const OatRope* rope, const void* turned, int M, int Hq, int Hkv) {
   if (rope && !turned && M) return fail(me, "rotary positions need a buffer for the turned queries and keys");
