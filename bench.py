@@ -28,6 +28,12 @@ sys.path.insert(0, ROOT)
 # stack.  Must be in the environment before the HIP runtime initialises, i.e. before torch touches the GPU.
 os.environ.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")
 
+# launcher test hook: what this rank was started with, before anything slow (a rank that fails first has the others stopped)
+if os.environ.get("OAT_BENCH_ECHO_RANK") == "1" and "RANK" in os.environ:
+    print(f"bench.py rank {os.environ['RANK']}/{os.environ.get('WORLD_SIZE')} LOCAL_RANK={os.environ.get('LOCAL_RANK')} "
+          f"MASTER_ADDR={os.environ.get('MASTER_ADDR')} MASTER_PORT={os.environ.get('MASTER_PORT')} "
+          f"HSA_ENABLE_IPC_MODE_LEGACY={os.environ.get('HSA_ENABLE_IPC_MODE_LEGACY')}", file=sys.stderr, flush=True)
+
 
 def _self_launch():
     """`python bench.py --gpus N` with N > 1 and NO launcher around it (no RANK / WORLD_SIZE in the environment):
@@ -584,9 +590,6 @@ def main():
     world = int(os.environ.get("WORLD_SIZE", 1))
     rank = int(os.environ.get("RANK", 0))
     local = int(os.environ.get("LOCAL_RANK", 0))
-    if os.environ.get("OAT_BENCH_ECHO_RANK") == "1":       # launcher test hook: what this rank was started with
-        print(f"bench.py rank {rank}/{world} LOCAL_RANK={local} MASTER_ADDR={os.environ.get('MASTER_ADDR')} MASTER_PORT={os.environ.get('MASTER_PORT')} "
-              f"HSA_ENABLE_IPC_MODE_LEGACY={os.environ.get('HSA_ENABLE_IPC_MODE_LEGACY')}", file=sys.stderr, flush=True)
     if not torch.cuda.is_available():
         raise SystemExit("bench.py needs an MI355X (no CPU path for the product)")
     if os.environ.get("OAT_BENCH_ONE_DEVICE") == "1":      # dry run of the N > 1 path on a one-GPU box (with OAT_BENCH_BACKEND=gloo)
