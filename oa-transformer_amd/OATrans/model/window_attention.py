@@ -170,12 +170,13 @@ class WindowCache:
         self.pieces = hip.window_step_workspace(B, heads, kv_heads, head_dim, self.k.device)
 
     @torch.no_grad()
-    def prompt(self, qkv, seqs, longest, pos=None, scale=None):
+    def prompt(self, qkv, seqs, longest=None, pos=None, scale=None):
         """Causal attention over the prompts; their keys and values and their counts go into the cache.  longest: the largest count of
-        the table; a sequence with more is taken as empty, here and in its counts."""
+        the table (default: all rows); a sequence with more is taken as empty, here and in its counts."""
+        longest = qkv.shape[0] if longest is None else min(int(longest), qkv.shape[0])
         out = window_attention(qkv, seqs, self.heads, self.kv_heads, self.head_dim, left=self.left, right=0, sinks=self.sinks,
                                longest=longest, scale=scale, rope=self.rope, pos=pos, cache=(self.k, self.v))
-        hip.window_cache_counts(self.past, seqs, qkv.shape[0], min(int(longest), qkv.shape[0]))
+        hip.window_cache_counts(self.past, seqs, qkv.shape[0], longest)
         return out
 
     @torch.no_grad()

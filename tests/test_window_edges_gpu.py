@@ -288,3 +288,47 @@ def test_fp16_gradients_up_to_the_limit_and_beyond(D, Hq, Hkv, n, sinks):
     other = torch.ones(n, dtype=torch.bool, device=DEV)
     other[at] = False
     assert torch.equal(got[0][other], ok[0][other])
+
+
+# ---------------------------------------------------------------------------------------------- a cache as a program uses it
+@pytest.mark.parametrize("window,slots,sinks", [(None, 40, 0), (6, None, 2)])
+def test_captured_prompts_and_steps_replay(window, slots, sinks):
+    """A prompt, and a step with its count, in HIP graphs of their own: replayed with new inputs, eager work between, against eager calls."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    Hq, Hkv, D, lens = 4, 2, 64, [9, 17, 1]
+    W, M, rope = (Hq + 2 * Hkv) * D, sum(lens), hip.RopeAxes((64,))
+    pos, table = torch.cat([torch.arange(n) for n in lens])[:, None].int().to(DEV), hip.seq_table(lens)
+    ours, other = (wa.WindowCache(3, Hq, Hkv, D, window=window, sinks=sinks, slots=slots, rope=rope) for _ in range(2))
+    qkv, x = torch.zeros(M, W, dtype=BF, device=DEV), torch.zeros(3, W, dtype=BF, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            ours.prompt(qkv, table, max(lens), pos=pos), ours.step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    first, then = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        read = ours.prompt(qkv, table, max(lens), pos=pos)
+    with torch.cuda.graph(then):
+        said = ours.step(x)
+    for k in range(3):
+        qkv.copy_(rnd(M, W, seed=60 + k))
+        first.replay()
+        assert torch.equal(read, other.prompt(qkv, table, max(lens), pos=pos)) and ours.past.tolist() == lens
+        for t in range(30):
+            x.copy_(rnd(3, W, seed=100 * k + t))
+            then.replay()
+            assert torch.equal(said, other.step(x)), (k, t)
+        assert torch.equal(ours.past, other.past) and torch.equal(ours.k, other.k) and torch.equal(ours.v, other.v)
+        full = [min(n + 30, slots) if slots else n + 30 for n in lens]
+        assert ours.past.tolist() == full
+
+
+def test_a_prompt_without_its_longest_count():
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    lens, qkv = [5, 12, 3], rnd(20, 192, seed=1)
+    a, b = wa.WindowCache(3, 1, 1, 64, slots=20), wa.WindowCache(3, 1, 1, 64, slots=20)
+    assert torch.equal(a.prompt(qkv, hip.seq_table(lens)), b.prompt(qkv, hip.seq_table(lens), 12))
+    assert a.past.tolist() == b.past.tolist() == lens and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
