@@ -1068,6 +1068,7 @@ def rope_axes(x, pos, rope, heads, head_dim, out=None, inverse=False):
     _need(pos.dtype == torch.int32 and pos.dim() == 2 and pos.shape[1] == rope.axes and pos.is_contiguous() and pos.device == x.device,
           f"rope_axes: pos must be a contiguous int32 [P, {rope.axes}] on {x.device}")
     M = x.shape[0]
+    _need(M < 2 ** 31, "rope_axes: x has 2^31 rows or more")
     if out is None:
         out = torch.empty(M, heads * head_dim, dtype=x.dtype, device=x.device)
     else:

@@ -190,3 +190,13 @@ def test_every_check_of_the_binding_says_what_is_wrong():
             pytest.fail(f"{name}: taken")
         count += 1
     assert count > 90
+
+
+def test_rows_beyond_32_bits_are_not_cut():
+    """2^32 + 8 rows of two values fit the card: they are refused, not taken for 8."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    x, rope, pos = torch.zeros(1, 2, dtype=torch.bfloat16).expand(2 ** 32 + 8, 2), hip.RopeAxes((2,)), torch.zeros(8, 1, dtype=torch.int32)
+    for call in (hip.rope_axes, wa.rope_axes):
+        with pytest.raises(hip.OatError, match="2.31 rows"):
+            call(x, pos, rope, 1, 2)
