@@ -305,8 +305,8 @@ int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dt
  * seqs: int32 [B, 4] on the device = (first query row, queries, first key row, keys) of every sequence - packed, padded or of different
  * query and key counts; query i stands at p = i + keys - queries and sees key j if  j <= p + right  and  (j >= p - left or j < sinks);
  * left / right < 0: no such edge (right = 0: causal).  A row that sees nothing gives 0 and lse = -inf (only such a row does: where a score
- * is not a number, out and lse are none either).  Rows of no sequence are left as they were.  A sequence that does not fit rows_q / rows_k / max_q / max_k is taken as empty.  lse: fp32 [rows_q, Hq] (natural
- * logarithm) or NULL.  Rows of a sequence have to be finite: what a masked pair holds is multiplied by an exact zero. */
+ * is not a number, out and lse are none either).  Rows of no sequence are left as they were.  A sequence that does not fit rows_q /
+ * rows_k / max_q / max_k is taken as empty.  lse: fp32 [rows_q, Hq] (natural logarithm) or NULL.  Rows of a sequence have to be finite: what a masked pair holds is multiplied by an exact zero. */
 int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
                         float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
                         int left, int right, int sinks, float scale, void* stream);
@@ -339,14 +339,21 @@ int oat_window_cache_advance(int* past, int B, int cap, void* stream);
 
 /* The layer on packed rows qkv [M, (Hq + 2 Hkv) * D] (q | k | v), one call each way.  Forward: rotary positions of q and k into
  * turned [M, (Hq + Hkv) * D] (rope NULL: turned unused; table, if not NULL: the cos and sin of every row's pairs, fp32 [n_pairs, M, 2]), attention with the sequences' query rows as their key rows, out [M, Hq * D]
- * dense, and - with k_cache - the prompt's cache.  A sequence that is left out because it has more than `longest` tokens gets zeros, both
- * ways (but for longest = 0: nothing is written).  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back (with the forward's table, of
+ * dense, and - with k_cache - the prompt's cache.  Backward: dqkv [M, (Hq + 2 Hkv) * D] dense, turned back (with the forward's table, of
  * pairs that are a head's two halves, before its rounding; else in a pass of its own); workspace as for
  * oat_attn_window_bwd with max_q = max_k = longest. */
 int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out, float* lse,
                              const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks,
                              float scale, void* k_cache, void* v_cache, const long long* strides, int cap, void* stream);
 int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period, const void* out,
+                             const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D,
+                             int dtype, int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* The same where every row belongs to one sequence: a sequence that is left out, because it has more than `longest` (not 0) tokens, gets
+ * zeros, both ways. */
+int oat_window_attention_packed_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out, float* lse,
+                             const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks,
+                             float scale, void* k_cache, void* v_cache, const long long* strides, int cap, void* stream);
+int oat_window_attention_packed_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period, const void* out,
                              const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D,
                              int dtype, int left, int right, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -42,7 +42,7 @@ def rope_axes(x, pos, rope, heads, head_dim):
 
 
 def _new(packed, longest, seqs):
-    """how a result starts: the library writes the rows of every sequence whose rows lie in the buffer, where there is any work"""
+    """how a result starts: where every row belongs to a sequence the library writes them all, if there is any work"""
     return torch.empty if packed and longest > 0 and seqs.shape[0] else torch.zeros
 
 
@@ -74,7 +74,7 @@ def _forward(qkv, seqs, pos, heads, kv_heads, D, longest, window, scale, rope, p
         if k.dtype is not dt or k.device != dev or k.shape[0] != seqs.shape[0] or k.shape[2] != kv_heads or k.shape[3] != D:
             raise hip.OatError(f"{what}: the caches must be [{seqs.shape[0]}, slots, {kv_heads}, {D}] of {dt} on {dev}")
         kc, vc = k.data_ptr(), v.data_ptr()
-    hip._launch(dev, hip.lib().oat_window_attention_fwd, (
+    hip._launch(dev, hip.lib().oat_window_attention_packed_fwd if packed else hip.lib().oat_window_attention_fwd, (
         qkv.data_ptr(), hip._ld(qkv), turned, turns.data_ptr() if turns is not None else None, struct, places, period, out.data_ptr(), lse.data_ptr() if lse is not None else None,
         seqs.data_ptr(), seqs.shape[0], longest, M, heads, kv_heads, D, hip._ELEMENTS[dt], *window, D ** -0.5 if scale is None else scale,
         kc, vc, strides, cap), what)
@@ -105,7 +105,7 @@ class _WindowFn(torch.autograd.Function):
         dqkv = _new(packed, longest, seqs)(qkv.shape, dtype=qkv.dtype, device=dev)
         need = lib.oat_attn_window_bwd_workspace_bytes(M, B, longest, longest, heads, kv_heads, D, window[0], window[2])
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        hip._launch(dev, lib.oat_window_attention_bwd, (
+        hip._launch(dev, lib.oat_window_attention_packed_bwd if packed else lib.oat_window_attention_bwd, (
             qkv.data_ptr(), hip._ld(qkv), qk.data_ptr() if qk is not None else None,
             turns.data_ptr() if turns is not None else None, rope.struct if rope is not None else None,
             pos.data_ptr() if pos is not None else None, pos.shape[0] if pos is not None else 0, out.data_ptr(), lse.data_ptr(),

@@ -50,6 +50,8 @@ _WINDOW_SIGNATURES = {
     "oat_window_cache_counts": (_I, [_P, _P, _I, _I, _I, _P]),
     "oat_window_cache_advance": (_I, [_P, _I, _I, _P]),
 }
+for _way in ("fwd", "bwd"):
+    _WINDOW_SIGNATURES["oat_window_attention_packed_" + _way] = _WINDOW_SIGNATURES["oat_window_attention_" + _way]
 
 
 def lib():

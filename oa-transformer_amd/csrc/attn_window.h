@@ -141,7 +141,7 @@ struct WinArgs {
   int run;                              // tiles that go to one XCD together
   int groups, pieces, far_blocks;       // how the sinks' far queries are split; their workgroups in the launch
   float scale;
-  int clear;                            // rows of a sequence that is left out for its length get zeros (the layer's do)
+  int clear;                            // rows of a sequence that is left out for its length get zeros (the layer's on packed rows do)
   const float2* turns;                  // backward: cos and sin of [D / 2, rows_q] pairs (p, p + D / 2) to turn dq and dk back by, or null
 };
 struct Seq { int q0, nq, k0, nk; };
@@ -154,7 +154,7 @@ OAT_DEV Seq load_seq(const WinArgs& a, int b) {
   return left_out(a, s) ? Seq{0, 0, 0, 0} : Seq{s.x, s.y, s.z, s.w};
 }
 // Zeros for head h's rows of a sequence that load_seq left out though its rows lie in the buffer (there are more than stated, or its other
-// side does not fit): the caller's buffer may be a new one, and no other workgroup writes them.  `part` of `parts` workgroups.
+// side does not fit), for buffers in which every row is one sequence's: no other workgroup writes them.  `part` of `parts` workgroups.
 template <int D> OAT_DEV void clear_rows(char* base, long long ld, int first, int n, int rows, int h, int part, int parts) {
   if (!rows_fit(first, n, n, rows)) return;
   constexpr int CPR = D / 8;

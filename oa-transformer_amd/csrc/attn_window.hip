@@ -585,8 +585,8 @@ template <class T, int D> OAT_DEV void window_keys(const WinArgs& a, char* lds) 
 
 // The same for 64 keys, heads of 128: two waves share 32 keys.  Each forms P and dS of one half of a tile, hands one of them to the other
 // through the LDS, and then one adds up dV, the other dK, of the whole tile: every product is formed once, and a wave holds one sum
-// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above, with the sinks' far queries and the turn
-// back: 113 us = 488 TFLOP/s (matrix unit 29 %, vector unit 24 %, 1.4 waves on a SIMD).
+// instead of two (64 instead of 128 registers at D = 128), so that two waves fit a SIMD.  The packed texts of above, with the sinks' far
+// queries and the turn back: 113 us = 488 TFLOP/s (matrix unit 29 %, vector unit 24 %, 1.4 waves on a SIMD).
 template <class T, int D> OAT_DEV void window_keys_in_pairs(const WinArgs& a, char* lds) {
   constexpr int TB = TILE * D * 2, ST = 2 * TB + 512;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, G = a.Hq / a.Hkv;

@@ -49,7 +49,8 @@ template <int D> constexpr int step_lds() { return 4 * 2 * SK * D * 2; }
 // O^T += V^T P^T on 16x16x32 products with the query head as the column: shared heads cost nothing more than one.
 // The new token's query and key are turned here (one angle per pair and workgroup); the workgroup of the piece that holds the
 // new token writes its row to the cache first.  The turned query and key and the probabilities are rounded to the operands' 16 bits (the
-// cache holds no more, the matrix unit takes no more); scores, statistics and sums are 32-bit.  Pieces are joined by the workgroup that finishes last, in a fixed order.
+// cache holds no more, the matrix unit takes no more); scores, statistics and sums are 32-bit.  Pieces are joined by the workgroup that
+// finishes last, in a fixed order.
 // Measured: 64 sequences of up to 4096 tokens, 32 / 8 heads of 128: 576 MB in 117 us = 4.9 TB/s; two of 65536 visible tokens: 537 MB in
 // 107 us = 5.0 (a large copy: 4.9 to 5.4); one of 512, 12 heads of 64: 7.8 us, a chain of dependent loads.
 template <class T, int D>
@@ -475,6 +476,7 @@ extern "C" int oat_window_cache_advance(int* past, int B, int cap, void* stream)
 
 // ---- what a layer on packed q | k | v rows does, in one call each way (one crossing into the library instead of three).  The turned q and k
 // are held in the rows' type: the matrix unit takes no more, and the cache keeps the keys as they are
+
 // whether the gradient's way back through the rotary positions is taken where dq and dk are formed.  A pair's two values have to meet in one
 // lane: those of a head's two halves do, in one register of two fragments, and this is the ladder that has the code.  (So would neighbours,
 // and halves of fewer pairs that are a multiple of 8: such ladders take a pass of their own and round twice.)
@@ -485,9 +487,9 @@ static int packed_wrong(const char* me, const OatRope* rope, const void* turned,
   return 0;
 }
 
-extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out,
+static int layer_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out,
                                         float* lse, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left,
-                                        int right, int sinks, float scale, void* kc, void* vc, const long long* strides, int cap, void* stream) {
+                                        int right, int sinks, float scale, void* kc, void* vc, const long long* strides, int cap, int clear, void* stream) {
   if (int rc = packed_wrong("window_attention_fwd", rope, turned, M, Hq, Hkv)) return rc;
   const long long n = (long long)(Hq + Hkv) * D, a = (long long)Hq * D;
   const char* q = (const char*)qkv;
@@ -500,14 +502,14 @@ extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* tur
   }
   const char* k = M ? q + a * 2 : q;
   if (int rc = attn_window_fwd(q, ldq, k, ldq, v, ld, out, a, lse, seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks,
-                               scale, 1, stream)) return rc;
+                               scale, clear, stream)) return rc;
   return kc ? cache_fill(k, ldq, v, ld, seqs, B, M, longest, M, longest, kc, vc, strides, cap, Hkv, D, sinks, stream) : 0;
 }
 
-extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period,
+static int layer_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period,
                                         const void* out, const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest,
                                         int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
+                                        size_t workspace_bytes, int clear, void* stream) {
   if (int rc = packed_wrong("window_attention_bwd", rope, turned, M, Hq, Hkv)) return rc;
   if (M == 0) return 0;
   const long long n = (long long)(Hq + Hkv) * D, a = (long long)Hq * D, w = n + (long long)Hkv * D;
@@ -520,6 +522,33 @@ extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const voi
   if (turns && (uintptr_t)table % 8) return fail("window_attention_bwd", "the table of the turns is not aligned to 8 bytes");
   if (int rc = attn_window_bwd(q, ldq, q + a * 2, ldq, (const char*)qkv + n * 2, ld, out, a, lse, dout, a, g, w, g + a * 2, w, g + n * 2, w,
                                    seqs, B, longest, longest, M, M, Hq, Hkv, D, dtype, left, right, sinks, scale, workspace, workspace_bytes,
-                               turns, 1, stream)) return rc;
+                               turns, clear, stream)) return rc;
   return rope && !turns ? oat_rope_axes(g, w, g, w, dtype, pos, period, M, Hq + Hkv, D, rope, 1, stream) : 0;
+}
+
+extern "C" int oat_window_attention_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out,
+                                        float* lse, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left,
+                                        int right, int sinks, float scale, void* kc, void* vc, const long long* strides, int cap, void* stream) {
+  return layer_fwd(qkv, ld, turned, table, rope, pos, period, out, lse, seqs, B, longest, M, Hq, Hkv, D, dtype, left, right, sinks, scale, kc, vc, strides,
+                   cap, 0, stream);
+}
+extern "C" int oat_window_attention_packed_fwd(const void* qkv, long long ld, void* turned, float* table, const OatRope* rope, const int* pos, int period, void* out,
+                                        float* lse, const int* seqs, int B, int longest, int M, int Hq, int Hkv, int D, int dtype, int left,
+                                        int right, int sinks, float scale, void* kc, void* vc, const long long* strides, int cap, void* stream) {
+  return layer_fwd(qkv, ld, turned, table, rope, pos, period, out, lse, seqs, B, longest, M, Hq, Hkv, D, dtype, left, right, sinks, scale, kc, vc, strides,
+                   cap, 1, stream);
+}
+extern "C" int oat_window_attention_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period,
+                                        const void* out, const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest,
+                                        int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  return layer_bwd(qkv, ld, turned, table, rope, pos, period, out, lse, dout, dqkv, seqs, B, longest, M, Hq, Hkv, D, dtype, left, right, sinks, scale,
+                   workspace, workspace_bytes, 0, stream);
+}
+extern "C" int oat_window_attention_packed_bwd(const void* qkv, long long ld, const void* turned, const float* table, const OatRope* rope, const int* pos, int period,
+                                        const void* out, const float* lse, const void* dout, void* dqkv, const int* seqs, int B, int longest,
+                                        int M, int Hq, int Hkv, int D, int dtype, int left, int right, int sinks, float scale, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  return layer_bwd(qkv, ld, turned, table, rope, pos, period, out, lse, dout, dqkv, seqs, B, longest, M, Hq, Hkv, D, dtype, left, right, sinks, scale,
+                   workspace, workspace_bytes, 1, stream);
 }

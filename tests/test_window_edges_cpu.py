@@ -200,3 +200,14 @@ def test_rows_beyond_32_bits_are_not_cut():
     for call in (hip.rope_axes, wa.rope_axes):
         with pytest.raises(hip.OatError, match="2.31 rows"):
             call(x, pos, rope, 1, 2)
+
+
+@pytest.mark.parametrize("change,text", [(dict(D=96), b"64 or 128"), (dict(Hkv=0), b"no heads"), (dict(longest=-1), b"lengths"), (dict(scale=0.0), b"scale"), (dict(seqs=None), b"table")])
+def test_packed_layer_refusals(change, text):
+    from tests.test_window_cpu import LAYER
+    hip = _hip()
+    a = {**LAYER, **change}
+    _refused(hip, hip.lib().oat_window_attention_packed_fwd(*a.values(), None), text)
+    head = [a[n] for n in ("qkv", "ld", "turned", "table", "rope", "pos", "period", "out")] + [4096, 4096, 4096]
+    tail = [a[n] for n in ("seqs", "B", "longest", "M", "Hq", "Hkv", "D", "dtype", "left", "right", "sinks", "scale")]
+    _refused(hip, hip.lib().oat_window_attention_packed_bwd(*head, *tail, 4096, 1 << 40, None), text)

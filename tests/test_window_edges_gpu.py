@@ -332,3 +332,18 @@ def test_a_prompt_without_its_longest_count():
     a, b = wa.WindowCache(3, 1, 1, 64, slots=20), wa.WindowCache(3, 1, 1, 64, slots=20)
     assert torch.equal(a.prompt(qkv, hip.seq_table(lens)), b.prompt(qkv, hip.seq_table(lens), 12))
     assert a.past.tolist() == b.past.tolist() == lens and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+
+
+def test_a_sequence_that_is_left_out_does_not_touch_its_neighbours():
+    """A padded batch whose table claims a row too many: that sequence is left out, the next one, whose first row it claims, is not harmed."""
+    hip = _hip()
+    from OATrans.model import window_attention as wa
+    L, D = 300, 64
+    qkv, dout = rnd(4 * L, 3 * D, seed=1).requires_grad_(), rnd(4 * L, D, seed=2)
+    lens = [L, L + 1, L, 40]
+    table, ok = hip.seq_table(lens, q_rows=range(0, 4 * L, L)), hip.seq_table([L, 0, L, 40], q_rows=range(0, 4 * L, L))
+    for _ in range(20):
+        out = wa.window_attention(qkv, table, 1, 1, D, longest=L)
+        ref = wa.window_attention(qkv, ok, 1, 1, D, longest=L)
+        assert torch.equal(out, ref)
+        assert torch.equal(torch.autograd.grad(out, qkv, dout)[0], torch.autograd.grad(ref, qkv, dout)[0])
