@@ -306,7 +306,8 @@ int oat_rope_axes(const void* x, long long ldx, void* out, long long ldo, int dt
  * query and key counts; query i stands at p = i + keys - queries and sees key j if  j <= p + right  and  (j >= p - left or j < sinks);
  * left / right < 0: no such edge (right = 0: causal).  A row that sees nothing gives 0 and lse = -inf (only such a row does: where a score
  * is not a number, out and lse are none either).  Rows of no sequence are left as they were.  A sequence that does not fit rows_q /
- * rows_k / max_q / max_k is taken as empty.  lse: fp32 [rows_q, Hq] (natural logarithm) or NULL.  Rows of a sequence have to be finite: what a masked pair holds is multiplied by an exact zero. */
+ * rows_k / max_q / max_k is taken as empty.  lse: fp32 [rows_q, Hq] (natural logarithm) or NULL.  Rows of a sequence have to be finite:
+ * what a masked pair holds is multiplied by an exact zero. */
 int oat_attn_window_fwd(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out, long long ldo,
                         float* lse, const int* seqs, int B, int max_q, int max_k, int rows_q, int rows_k, int Hq, int Hkv, int D, int dtype,
                         int left, int right, int sinks, float scale, void* stream);
